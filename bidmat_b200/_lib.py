@@ -12,6 +12,8 @@ LIBPATH = os.path.join(_PKG, "lib", "libbidmatcuda_b200.so")
 HEADER = os.path.join(_PKG, "..", "include", "bidmat_b200.h")
 
 _c_int = ctypes.c_int
+_c_ll = ctypes.c_longlong
+_c_float = ctypes.c_float
 _vp = ctypes.c_void_p
 
 # name -> (restype, argtypes); pointers travel as integers (device addresses).
@@ -71,6 +73,17 @@ _SIGNATURES = {
     "bidmat_b200_sdoprow_f64": (_c_int, [_c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int]),
     "bidmat_b200_sdopcol_f64": (_c_int, [_c_int, _c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int]),
     "bidmat_b200_check_structure": (_c_int, [_c_int, _c_int, _c_int, _vp, _vp]),
+    "bidmat_b200_route": (_c_int, [_c_int, _c_int, _vp, _c_ll, _c_int, _c_int, _c_int, _vp, _c_int, _c_int, _c_int, _c_int,
+                                   _c_float, _vp, _vp, _vp, _vp, _vp]),
+    "bidmat_b200_route_grad": (_c_int, [_c_int, _c_int, _c_int, _vp, _c_ll, _c_int, _c_int, _c_int, _c_float, _vp, _vp, _vp,
+                                        _vp, _vp, _c_ll, _vp]),
+    "bidmat_b200_top_logits": (_c_int, [_c_int, _c_int, _vp, _c_ll, _c_int, _c_int, _c_float, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "bidmat_b200_distill": (_c_int, [_c_int, _c_int, _c_int, _vp, _c_ll, _c_int, _c_float, _vp, _vp, _vp, _vp, _vp, _vp,
+                                     _vp]),
+    "bidmat_b200_distill_grad": (_c_int, [_c_int, _c_int, _c_int, _vp, _c_ll, _c_int, _c_float, _vp, _vp, _vp, _vp, _vp,
+                                          _vp, _vp, _c_ll, _vp]),
+    "bidmat_b200_distill_with_grad": (_c_int, [_c_int, _c_int, _c_int, _vp, _c_ll, _c_int, _c_float, _vp, _vp, _vp, _vp,
+                                               _vp, _vp, _vp, _c_ll, _vp]),
     "bidmat_b200_workspace_bytes": (ctypes.c_longlong, []),
     "bidmat_b200_release_workspace": (_c_int, []),
     "bidmat_b200_launch_count": (ctypes.c_longlong, []),

@@ -351,6 +351,39 @@ class GMat:
         return DDS(self, pair.left, pair.right, None)
 
 
+class GHMat:
+    """Dense matrix of 16-bit floats (bfloat16 or float16) on the device, column-major nrows x ncols:
+    the form in which a language model's logits, scores and their gradients arrive.  Only the operators
+    of bidmat_b200.tokens take it.  Backed by a torch tensor of shape (ncols, nrows) whose rows are
+    contiguous; they may lie further apart than nrows (a slice of a padded vocabulary)."""
+
+    def __init__(self, tensor):
+        if tensor.dtype not in (torch.bfloat16, torch.float16) or tensor.dim() != 2:
+            raise RuntimeError("GHMat needs a 2-D bfloat16 or float16 tensor (ncols, nrows)")
+        if tensor.shape[1] > 1 and tensor.stride(1) != 1 or tensor.shape[0] > 1 and tensor.stride(0) < tensor.shape[1]:
+            raise RuntimeError("GHMat needs contiguous columns that do not overlap")
+        if not tensor.is_cuda:
+            raise RuntimeError("GHMat data must live on a CUDA device (no CPU fallback)")
+        self.t = tensor
+
+    @property
+    def nrows(self):
+        return int(self.t.shape[1])
+
+    @property
+    def ncols(self):
+        return int(self.t.shape[0])
+
+    @property
+    def ld(self):
+        """Elements from one column to the next."""
+        return max(self.nrows, int(self.t.stride(0))) if self.ncols > 1 else self.nrows
+
+    @property
+    def pdata(self):
+        return self.t.data_ptr()
+
+
 class GDSPair:
     """GDSPair (GMat.scala:1978-1990)."""
 

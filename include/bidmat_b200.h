@@ -375,6 +375,96 @@ BIDMAT_B200_API int bidmat_b200_spsum_f64(int nrows, int ncols, int nnz, const i
  * Synchronous. */
 BIDMAT_B200_API int bidmat_b200_check_structure(int m, int ncols, int nnz, const int *ir, const int *ic);
 
+/* ---- Token columns and sparse matrices ----------------------------------------------------
+ * Operators of language models between dense matrices that hold one token per column and sparse
+ * matrices that hold a few rows of each token: routing to experts, a teacher's top logits, and the
+ * loss of a student against them.  The sparse results are ordinary GSMats: A*S mixes or combines the
+ * routed columns of A, B*^S is the gradient of A, DDS(A, dC, S) the gradient of the weights, the
+ * transpose lists the tokens of every expert.  No counterpart in the reference's native interface.
+ * Common to all of them:
+ *   - dense operands are column-major with a leading dimension ld >= nrows counted in elements; dtype
+ *     gives the element type.  Arithmetic is in 32 bits or more whatever the type and results are
+ *     rounded once.  Pointers are aligned to their elements; 16-byte aligned columns are read faster;
+ *   - everything is stream-ordered on `stream` and can be captured into a graph; no scratch memory;
+ *   - results are bit-reproducible (no float atomics);
+ *   - ncols == 0 succeeds; sizes and flags outside the stated ranges and null pointers return
+ *     cudaErrorInvalidValue before anything is launched. */
+#define BIDMAT_B200_F32 0
+#define BIDMAT_B200_BF16 1
+#define BIDMAT_B200_F16 2
+
+/* Routing: picks k of the nrows experts for every column of the scores X(nrows x ncols) and writes
+ * the sparse matrix S(nrows x ncols) of their weights with exactly k entries per column: Sir, Sic,
+ * Sdata hold k*ncols entries (k*ncols < 2^31), Sjc ncols+1.
+ *   s    = softmax over the column (score == BIDMAT_B200_SOFTMAX) or sigmoid (BIDMAT_B200_SIGMOID);
+ *   key  = s + bias[row]; with bias == NULL the order of the scores themselves.  The bias takes part in
+ *          the choice only, not in the weights;
+ *   groups: ngroups equal groups of consecutive rows.  A group counts as the sum of its `grouptop` (1 or
+ *          2) best s + bias; only the rows of the `topgroups` best groups compete (ties: lower group);
+ *   weight = s of the picked row, divided by the sum over the picked rows if renorm != 0, times scale.
+ * Entries come in descending order of their keys, equal keys by ascending row; keys are compared as in
+ * 64 bits.  A score or bias of -infinity (or a NaN bias) takes a row out; when fewer than k rows are
+ * left the column is filled up with the lowest other rows at weight 0 (all of them for a column of
+ * -infinity).  A column with a NaN or +infinity gets rows 0..k-1 and NaN weights.
+ * 1 <= nrows <= BIDMAT_B200_ROUTE_MAX_ROWS, 1 <= k <= BIDMAT_B200_ROUTE_MAX_K, k <= topgroups *
+ * nrows/ngroups, ngroups divides nrows; scale is finite and not 0. */
+#define BIDMAT_B200_SOFTMAX 0
+#define BIDMAT_B200_SIGMOID 1
+#define BIDMAT_B200_ROUTE_MAX_ROWS 1024
+#define BIDMAT_B200_ROUTE_MAX_K 32
+BIDMAT_B200_API int bidmat_b200_route(int nrows, int ncols, const void *X, long long ldx, int dtype, int k, int score,
+                                      const float *bias, int ngroups, int topgroups, int grouptop, int renorm,
+                                      float scale, int *Sir, int *Sic, int *Sjc, float *Sdata,
+                                      bidmat_stream_t stream);
+/* Its gradient: dX(nrows x ncols, of X's type) from the gradient dS of the weights (nnz values in the
+ * order of Sdata), with S as bidmat_b200_route left it for the same score, renorm and scale.  All of dX is
+ * written: rows that no entry names get 0, or, for a softmax without renorm, their share of the
+ * normalisation.  The choice itself and the bias have no gradient.  Columns may hold any number of entries;
+ * entries whose row is outside the matrix are left out.  dX may be X (with the same ld). */
+BIDMAT_B200_API int bidmat_b200_route_grad(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
+                                           int score, int renorm, float scale, const int *Sir, const int *Sjc,
+                                           const float *Sdata, const float *dS, void *dX, long long lddx,
+                                           bidmat_stream_t stream);
+
+/* The k largest logits of every column of X(nrows x ncols) as a sparse matrix S(nrows x ncols) with k
+ * entries per column (arrays as in bidmat_b200_route): the rows and the logits themselves, in descending
+ * order, equal logits by ascending row; NaN counts as larger than any number, -0 as equal to 0.
+ * lse (ncols values, may be NULL) receives log sum_v exp(X[v]/temperature) of every column.
+ * 1 <= k <= BIDMAT_B200_TOP_MAX_K, k <= nrows; temperature is finite and > 0. */
+#define BIDMAT_B200_TOP_MAX_K 512
+BIDMAT_B200_API int bidmat_b200_top_logits(int nrows, int ncols, const void *X, long long ldx, int dtype, int k,
+                                           float temperature, int *Sir, int *Sic, int *Sjc, float *Sdata, float *lse,
+                                           bidmat_stream_t stream);
+
+/* Distillation: Kullback-Leibler divergence of a student's logits X(nrows x ncols) from a teacher's top
+ * logits Z(nrows x ncols, sparse: Zir, Zjc, Zdata, any number of entries per column in any order), with
+ * t = temperature and, per column,
+ *     p_i  = exp(z_i/t - Lt),  Lt = Zlse[column], or, with Zlse == NULL, the log-sum-exp of the column's
+ *            entries z_i/t (p then sums to one over the entries),
+ *     L    = log sum_v exp(X[v]/t),
+ *     loss = sum_i p_i (log p_i - (X[row_i]/t - L)).
+ * distill writes loss and Xlse = L (ncols values each).
+ * distill_grad writes dX(nrows x ncols, of X's type), the gradient of sum_c weights[c] loss[c], from a
+ *     saved Xlse: dX[v] = weights/t (P exp(X[v]/t - L) - p_v) with P = sum p_i.
+ * distill_with_grad does both with one read of X; its loss is weights[c] loss[c] (the weights are known
+ *     before the loss: a mean over tokens, a loss mask, a loss scale).
+ * weights == NULL stands for ones.  Columns without an entry above -infinity have loss and gradient 0; so
+ * have columns of weight 0 in the two functions that take weights, which do not read them.  An entry
+ * whose row is outside the matrix makes its column's results NaN; a row that comes twice counts with the
+ * sum of its p.  A NaN or +infinity among a column's logits, or a column of -infinity, makes its results
+ * NaN (in fp32, so also in fp16 outputs; finite gradients above 65504 become infinite there). */
+BIDMAT_B200_API int bidmat_b200_distill(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
+                                        float temperature, const int *Zir, const int *Zjc, const float *Zdata,
+                                        const float *Zlse, float *loss, float *Xlse, bidmat_stream_t stream);
+BIDMAT_B200_API int bidmat_b200_distill_grad(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
+                                             float temperature, const int *Zir, const int *Zjc, const float *Zdata,
+                                             const float *Zlse, const float *Xlse, const float *weights, void *dX,
+                                             long long lddx, bidmat_stream_t stream);
+BIDMAT_B200_API int bidmat_b200_distill_with_grad(int nrows, int ncols, int nnz, const void *X, long long ldx,
+                                                  int dtype, float temperature, const int *Zir, const int *Zjc,
+                                                  const float *Zdata, const float *Zlse, const float *weights,
+                                                  float *loss, void *dX, long long lddx, bidmat_stream_t stream);
+
 /* Scratch memory.  Every call that needs scratch takes it from a memory pool the library
  * owns on the calling thread's device, by stream-ordered allocation on the call's stream,
  * and gives it back on that stream before returning; freed blocks stay cached in the pool
