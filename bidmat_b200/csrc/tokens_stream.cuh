@@ -1,0 +1,258 @@
+// Long columns read in 16-byte vectors, split over the CTAs of a cluster.
+//
+// A column of V elements starts at any element: it is treated as a row of 16-byte vectors from the aligned
+// address at or below its first element.  Position u = row + shift, shift = elements between that address and
+// the column; vector i holds the positions [i N, (i+1) N), N = 16 / sizeof(T).  Only the first and the last
+// vector can be partial; their elements are moved one by one, so nothing outside the column is touched.
+//
+// A thread keeps (m, s): the largest x so far and the sum of exp((x - m)/t) over its rows, taken as
+// 2^((x - m) c), c = log2(e)/t.  The difference comes first, so a column of the type's lowest value (a mask
+// that leaves nothing) neither overflows nor loses its uniform distribution.
+#pragma once
+#include <cooperative_groups.h>
+
+#include "tokens_common.cuh"
+
+namespace bidmat {
+
+constexpr double kLog2e = 1.4426950408889634074;
+constexpr double kLn2 = 0.69314718055994530942;
+
+__device__ __forceinline__ float exp2_fast(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// N elements of one 16-byte vector as floats and back.
+template <typename T> struct Pack;
+template <> struct Pack<float> {
+    static constexpr int N = 4;
+    static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
+        v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[N]) {
+        return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+    }
+    static __device__ __forceinline__ float max(const uint4 &r) {
+        return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
+    }
+};
+template <> struct Pack<__nv_bfloat16> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
+        const unsigned w[4] = {r.x, r.y, r.z, r.w};
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            v[2 * i] = __uint_as_float(w[i] << 16);
+            v[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[N]) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned *>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ float max(const uint4 &r) {
+        const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&r);
+        const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+};
+template <> struct Pack<__half> {
+    static constexpr int N = 8;
+    static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
+        const __half2 *p = reinterpret_cast<const __half2 *>(&r);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float2 f = __half22float2(p[i]);
+            v[2 * i] = f.x;
+            v[2 * i + 1] = f.y;
+        }
+    }
+    static __device__ __forceinline__ uint4 pack(const float (&v)[N]) {
+        unsigned w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const __half2 p = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+            w[i] = *reinterpret_cast<const unsigned *>(&p);
+        }
+        return make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    static __device__ __forceinline__ float max(const uint4 &r) {
+        const __half2 *p = reinterpret_cast<const __half2 *>(&r);
+        const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+};
+
+// Plain (coherent) loads: in place, the same kernel writes the column.
+__device__ __forceinline__ void store16(void *p, const uint4 &r) {
+    asm volatile("st.global.v4.u32 [%0], {%1,%2,%3,%4};" ::"l"(p), "r"(r.x), "r"(r.y), "r"(r.z), "r"(r.w) : "memory");
+}
+__device__ __forceinline__ uint4 load16(const void *p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p)
+                 : "memory");
+    return r;
+}
+
+// One column as vectors.
+template <typename T> struct Column {
+    static constexpr int N = Pack<T>::N;
+    const T *base;      // aligned address of vector 0
+    int shift, rows, nvec;
+    int full0, full1;   // the vectors that are the column's alone; before and behind at most one each is partial
+    __device__ __forceinline__ Column(const T *x, int nrows) : rows(nrows) {
+        shift = (int)((reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T));
+        base = x - shift;
+        const long long end = (long long)shift + nrows;
+        nvec = (int)((end + N - 1) / N);
+        full0 = shift ? 1 : 0;
+        full1 = (int)(end / N);
+        if (full1 < full0) full1 = full0;       // everything inside the first vector
+    }
+    // position j of vector i belongs to the column
+    __device__ __forceinline__ bool inside(int i, int j) const {
+        const long long u = (long long)i * N + j;
+        return u >= shift && u < (long long)shift + rows;
+    }
+    __device__ __forceinline__ uint4 load(int i) const { return load16(base + (long long)i * N); }
+    // a partial vector, -infinity where it is not the column's
+    __device__ __forceinline__ uint4 load_partial(int i) const {
+        float v[N];
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = inside(i, j) ? to_float(base[(long long)i * N + j]) : -INFINITY;
+        return Pack<T>::pack(v);
+    }
+    // The partial vectors among [v0, v1): number 0 and 1, or -1.
+    __device__ __forceinline__ int partial(int number, int v0, int v1) const {
+        const int i = number == 0 ? 0 : nvec - 1;
+        if (i >= full0 && i < full1) return -1;
+        if (number == 1 && i == 0 && full0 > 0) return -1;          // one vector, counted as the first
+        if (number == 0 && full0 == 0) return -1;                   // the first is full; the last is number 1
+        return i >= v0 && i < v1 ? i : -1;
+    }
+};
+
+// The two halves of a cluster-wide barrier.
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
+struct SumExp {
+    float m = -INFINITY, s = 0.f;
+    // what is subtracted: m, or 0 while everything was -infinity (the sum is then 0)
+    __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
+    __device__ __forceinline__ void raise(float top, float c) {
+        s = s == 0.f ? 0.f : s * exp2_fast((m - top) * c);       // a NaN stays
+        m = top;
+    }
+};
+
+// Two floats per instruction.
+__device__ __forceinline__ unsigned long long pair(float a, float b) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1,%2};" : "=l"(r) : "f"(a), "f"(b));
+    return r;
+}
+__device__ __forceinline__ float2 unpair(unsigned long long r) {
+    float2 v;
+    asm("mov.b64 {%0,%1}, %2;" : "=f"(v.x), "=f"(v.y) : "l"(r));
+    return v;
+}
+__device__ __forceinline__ unsigned long long add2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigned long long b) {
+    unsigned long long r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+// 2^((a - ref) c), 2^((b - ref) c)
+__device__ __forceinline__ float2 exp_pair(float a, float b, unsigned long long minus_ref, unsigned long long cc) {
+    const float2 e = unpair(mul2(add2(pair(a, b), minus_ref), cc));
+    return make_float2(exp2_fast(e.x), exp2_fast(e.y));
+}
+
+template <typename T> __device__ __forceinline__ void add_vector(SumExp &a, const uint4 &r, float c) {
+    constexpr int N = Pack<T>::N;
+    const float top = Pack<T>::max(r);
+    if (top > a.m) a.raise(top, c);
+    float v[N];
+    Pack<T>::unpack(r, v);
+    const float ref = a.ref();
+    const unsigned long long mr = pair(-ref, -ref), cc = pair(c, c);
+    unsigned long long acc = pair(0.f, 0.f);
+#pragma unroll
+    for (int j = 0; j < N; j += 2) {
+        const float2 e = exp_pair(v[j], v[j + 1], mr, cc);
+        acc = add2(acc, pair(e.x, e.y));
+    }
+    const float2 e = unpair(acc);
+    a.s += e.x + e.y;
+}
+
+// Both partners of an exchange get the same bits: the smaller maximum is always brought up to the larger one.
+__device__ __forceinline__ void join(SumExp &a, float m, float s, float c) {
+    if (m > a.m) {
+        a.raise(m, c);
+        a.s += s;
+    } else {
+        a.s += s == 0.f ? 0.f : (m == a.m ? s : s * exp2_fast((m - a.m) * c));
+    }
+}
+__device__ __forceinline__ void warp_join(SumExp &a, float c) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) {
+        const float m = __shfl_xor_sync(0xffffffffu, a.m, o), s = __shfl_xor_sync(0xffffffffu, a.s, o);
+        join(a, m, s, c);
+    }
+}
+
+// The vectors [v0, v1) of a column, four loads in flight per thread.
+template <typename T, int THREADS>
+__device__ __forceinline__ SumExp sum_exp_slice(const Column<T> &x, int v0, int v1, float c) {
+    constexpr int U = 4;
+    SumExp a;
+    const int f1 = min(v1, x.full1);
+    int i = max(v0, x.full0) + (int)threadIdx.x;
+    for (; i < f1 - (U - 1) * THREADS; i += U * THREADS) {
+        uint4 r[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) r[u] = x.load(i + u * THREADS);
+#pragma unroll
+        for (int u = 0; u < U; u++) add_vector<T>(a, r[u], c);
+    }
+    for (; i < f1; i += THREADS) add_vector<T>(a, x.load(i), c);
+    if (threadIdx.x < 2) {
+        const int p = x.partial((int)threadIdx.x, v0, v1);
+        if (p >= 0) add_vector<T>(a, x.load_partial(p), c);
+    }
+    return a;
+}
+
+// ------------------------------------------------------------------ host side
+// Clusters of `size` CTAs along x.
+inline cudaLaunchConfig_t cluster_config(cudaLaunchAttribute *attr, unsigned grid, unsigned threads, int size, size_t smem,
+                                         cudaStream_t st) {
+    attr->id = cudaLaunchAttributeClusterDimension;
+    attr->val.clusterDim.x = (unsigned)size;
+    attr->val.clusterDim.y = 1;
+    attr->val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cfg;
+}
+
+}  // namespace bidmat

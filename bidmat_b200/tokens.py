@@ -178,7 +178,7 @@ def distill(X, Z, temperature=1.0, lse=None):
 
 def distillGrad(X, Z, slse, weights=None, temperature=1.0, lse=None, omat=None):
     """The gradient in X of the sum over the tokens of weights * distill(X, Z, temperature, lse)[0], from the
-    log-sum-exp `slse` that distill returned."""
+    log-sum-exp `slse` that distill returned.  `omat` may be X."""
     what = "distillGrad"
     X, ld, dt = _dense(X, what)
     _sparse(Z, X, what)
@@ -195,7 +195,7 @@ def distillGrad(X, Z, slse, weights=None, temperature=1.0, lse=None, omat=None):
 
 def distillWithGrad(X, Z, weights=None, temperature=1.0, lse=None, omat=None):
     """(weights * loss, gradient of its sum in X) with one read of X: the training step's form, for weights
-    that are known before the loss (a mean over the tokens, a mask, a loss scale)."""
+    that are known before the loss (a mean over the tokens, a mask, a loss scale).  `omat` may be X."""
     what = "distillWithGrad"
     X, ld, dt = _dense(X, what)
     _sparse(Z, X, what)

@@ -452,7 +452,8 @@ BIDMAT_B200_API int bidmat_b200_top_logits(int nrows, int ncols, const void *X, 
  * have columns of weight 0 in the two functions that take weights, which do not read them.  An entry
  * whose row is outside the matrix makes its column's results NaN; a row that comes twice counts with the
  * sum of its p.  A NaN or +infinity among a column's logits, or a column of -infinity, makes its results
- * NaN (in fp32, so also in fp16 outputs; finite gradients above 65504 become infinite there). */
+ * NaN (in fp32, so also in fp16 outputs; finite gradients above 65504 become infinite there).
+ * dX may be X (with the same ld). */
 BIDMAT_B200_API int bidmat_b200_distill(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
                                         float temperature, const int *Zir, const int *Zjc, const float *Zdata,
                                         const float *Zlse, float *loss, float *Xlse, bidmat_stream_t stream);

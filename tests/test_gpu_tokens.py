@@ -404,6 +404,24 @@ def test_distill_sizes_and_types(cuda_device, dtype, V, T, k):
     check_distill(x, jc, ir, z, dtype, cuda_device, tau=1.0, tlse=tlse)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("V,T,k", [(5, 3, 5), (999, 40, 64), (70001, 3, 700), (300007, 2, 5)])
+def test_distill_gradient_in_place(cuda_device, dtype, V, T, k):
+    rng = np.random.default_rng(V)
+    jc, ir, z = teacher(rng, V, rng.integers(0, k + 1, T))
+    ir[::7] = ir[0]                                    # rows twice
+    Z = sparse(V, T, jc, ir, z, cuda_device)
+    for pad in (0, 3):
+        X = dense(rng.standard_normal((T, V)), dtype, cuda_device, pad)
+        loss, want = tokens.distillWithGrad(X, Z, temperature=2.0)
+        _, L = tokens.distill(X, Z, temperature=2.0)
+        want2 = tokens.distillGrad(X, Z, L, temperature=2.0)
+        Y = type(X)(X.t.clone(memory_format=torch.preserve_format))
+        assert tokens.distillGrad(Y, Z, L, temperature=2.0, omat=Y) is Y and same_bits(Y.t, want2.t)
+        loss2, dX = tokens.distillWithGrad(X, Z, temperature=2.0, omat=X)
+        assert dX is X and same_bits(X.t, want.t) and same_bits(loss.t, loss2.t)
+
+
 def test_distill_masks_and_infinities(cuda_device):
     rng = np.random.default_rng(12)
     V, n = 5003, 12
@@ -421,6 +439,7 @@ def test_distill_masks_and_infinities(cuda_device):
     z[jc[7]:jc[7] + 5] = -np.inf
     x[8, ir[jc[8]]] = -np.inf                          # a row the teacher wants and the student forbids
     x[9] = 80.0 * np.sign(x[9])
+    x[10] = low                                        # a mask of the lowest value that leaves nothing: uniform
     weights = np.ones(n, np.float32)
     weights[2] = 0.0                                   # the NaN column carries no weight
     check_distill(x, jc, ir, z, "fp32", cuda_device, weights=weights)
