@@ -19,7 +19,6 @@ namespace cg = cooperative_groups;
 namespace {
 
 constexpr int kStream = 256;              // threads that go over the rows; one more warp looks after the teacher
-constexpr int kThreadsAll = kStream + 32;
 constexpr int kMarkRows = 32768;          // rows per stretch of a gradient: one mark bit each
 
 struct Teacher {
@@ -28,137 +27,220 @@ struct Teacher {
     int nnz;
 };
 
-// A column's entries and what they amount to.
+// What a column's entries amount to.
 struct Entries {
-    int j0, j1;
     double lt, P;      // log-sum-exp and mass; P = 0: nothing to learn from, P = NaN: a row outside the matrix
     double cross;      // sum p (z - x)/t
 };
 
-// By one warp; x may be null when the loss is not wanted.
-template <typename T>
-__device__ __forceinline__ Entries read_entries(const Teacher &z, int j0, int j1, long long c, int nrows, double t, const T *x) {
+// Entries that a warp has in registers: the first 32 R of a column.
+constexpr int R = 4;
+struct Held {
+    int j0, j1;
+    int row[R];         // -1: none
+    float z[R];
+};
+__device__ __forceinline__ void hold(Held &h, const Teacher &z, int j0, int j1) {
     const int lane = threadIdx.x & 31;
-    Entries e;
-    e.j0 = j0;
-    e.j1 = j1;
-    if (z.lse) {
-        e.lt = z.lse[c];
-    } else {
-        double m = -INFINITY, s = 0.0;
-        for (int j = j0 + lane; j < j1; j += 32) m = max_nan(m, z.data[j] / t);
+    h.j0 = j0;
+    h.j1 = j1;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const int j = j0 + 32 * r + lane;
+        h.z[r] = j < j1 ? z.data[j] : -INFINITY;
+        h.row[r] = j < j1 ? z.ir[j] : -1;
+    }
+}
+
+// By one warp.  x: the student's column, read WITH_X.  xr, pr: the student's logits and the masses of the
+// entries held.  One exponential each.
+template <typename T, bool WITH_X>
+__device__ __forceinline__ Entries weigh_entries(const Held &h, const Teacher &z, long long c, int nrows, double t, const T *x,
+                                                 float (&xr)[R], float (&pr)[R]) {
+    const int lane = threadIdx.x & 31;
+    double shift = 0.0;
+    if (z.lse) shift = z.lse[c];
+    bool outside = false;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        const bool in = h.row[r] >= 0 && h.row[r] < nrows;
+        outside |= !in && h.j0 + 32 * r + lane < h.j1;
+        xr[r] = WITH_X && in ? to_float(x[h.row[r]]) : 0.f;
+    }
+    const int rest = h.j0 + 32 * R + lane;
+    if (!z.lse) {
+        double m = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; r++) m = max_nan(m, (double)h.z[r]);
+        for (int j = rest; j < h.j1; j += 32) m = max_nan(m, (double)z.data[j]);
         m = warp_max(m);
-        const double u = m == -INFINITY ? 0.0 : m;
-        for (int j = j0 + lane; j < j1; j += 32) s += exp(z.data[j] / t - u);
-        s = warp_sum(s);
-        e.lt = s == 0.0 ? INFINITY : u + log(s);       // nothing finite: every p is zero
+        shift = m == -INFINITY ? 0.0 : m / t;
     }
-    e.P = e.cross = 0.0;
-    for (int j = j0 + lane; j < j1; j += 32) {
-        const int row = z.ir[j];
-        const double p = (row >= 0 && row < nrows) ? exp(z.data[j] / t - e.lt) : NAN;
-        e.P += p;
-        if (x && p > 0.0) e.cross += p * (((double)z.data[j] - (double)to_float(x[row])) / t);
+    double s = 0.0, cross = 0.0;
+    auto add = [&](float zj, float xj) {
+        const double e = exp(zj / t - shift);
+        s += e;
+        if (WITH_X && e > 0.0) cross += e * (((double)zj - (double)xj) / t);
+        return e;
+    };
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        pr[r] = 0.f;
+        if (h.j0 + 32 * r < h.j1) pr[r] = (float)add(h.z[r], xr[r]);
     }
-    e.P = warp_sum(e.P);
-    e.cross = warp_sum(e.cross);
+    for (int j = rest; j < h.j1; j += 32) {
+        const int rj = z.ir[j];
+        const bool in = rj >= 0 && rj < nrows;
+        outside |= !in;
+        add(z.data[j], WITH_X && in ? to_float(x[rj]) : 0.f);
+    }
+    s = warp_sum(s);
+    if (WITH_X) cross = warp_sum(cross);
+    outside = __any_sync(0xffffffffu, outside);
+    Entries e;
+    if (z.lse) {
+        e.lt = shift;
+        e.P = s;
+        e.cross = cross;
+    } else {
+        e.lt = s == 0.0 ? INFINITY : shift + log(s);       // nothing finite: every p is zero
+        e.P = s == 0.0 ? 0.0 : s / s;                       // one, or NaN
+        e.cross = cross / s;
+#pragma unroll
+        for (int r = 0; r < R; r++) pr[r] = s == 0.0 ? 0.f : pr[r] / (float)s;
+    }
+    if (outside) e.P = e.cross = NAN;
     return e;
 }
 
-// Rows of the vectors [v0, v1) of the gradient: f exp((x - ref)/t) everywhere, and w/t (P q - p) at the
-// teacher's rows, q = exp((x - ref)/t) qf.  The rows with an entry are marked first, written by the threads of the entries, and
-// left out by the threads that go over the rows; so the column may be overwritten in place.
+// What the gradient of a column is made of: f exp((x - ref)/t) at every row, w/t (P qf exp((x - ref)/t) - p) at
+// the teacher's.
+struct Slope {
+    float t, c, w, ref, f;
+    double qf, lt, P;
+};
+
+// One stretch of the gradient is the vectors [a0, a1) of a column, at most kMarkRows rows.  The rows with an
+// entry are marked first, are written by the threads that have the entries and left out by those that
+// go over the rows; so the column may be overwritten in place (what a vector holds at a marked row is not used).
+
+// A barrier of the first THREADS threads only.
+template <int THREADS> __device__ __forceinline__ void sync_first() { asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory"); }
+
+// The first THREADS threads mark the stretch's entries; `twice` is set when a row comes twice.  To be seen by
+// others after a barrier.
 template <typename T, int THREADS>
-__device__ __forceinline__ void write_gradient(const Column<T> &x, T *dx, const Teacher &z, const Entries &e, int v0, int v1,
-                                               double t, double w, float ref, double qf, float f, float c, unsigned *marks) {
+__device__ __forceinline__ void mark_entries(const Column<T> &x, const Teacher &z, int j0, int j1, int a0, int a1, unsigned *marks,
+                                             int *twice) {
+    constexpr int N = Pack<T>::N;
+    const int tid = threadIdx.x;
+    for (int i = tid; i < (a1 - a0) * N / 32 + 1; i += THREADS) marks[i] = 0;
+    if (tid == 0) *twice = 0;
+    sync_first<THREADS>();
+    for (int j = j0 + tid; j < j1; j += THREADS) {
+        const int row = z.ir[j];
+        const long long u = (long long)row + x.shift - (long long)a0 * N;
+        if (row < 0 || row >= x.rows || u < 0 || u >= (long long)(a1 - a0) * N) continue;
+        if ((atomicOr(&marks[u >> 5], 1u << (u & 31)) >> (u & 31)) & 1u) *twice = 1;
+    }
+}
+
+// The rows with an entry, by `count` threads of which this is number `who`.
+template <typename T>
+__device__ __forceinline__ void write_entries(const Column<T> &x, T *out, const Teacher &z, int j0, int j1, int a0, int a1,
+                                              const Slope &g, bool twice, int who, int count) {
+    constexpr int N = Pack<T>::N;
+    const double t = g.t;
+    for (int j = j0 + who; j < j1; j += count) {
+        const int row = z.ir[j];
+        const long long u = (long long)row + x.shift - (long long)a0 * N;
+        if (row < 0 || row >= x.rows || u < 0 || u >= (long long)(a1 - a0) * N) continue;
+        double p = exp(z.data[j] / t - g.lt);
+        if (twice) {                                    // a row's first entry adds them up in their order
+            bool mine = true;
+            p = 0.0;
+            for (int i = j0; i < j1; i++)
+                if (z.ir[i] == row) {
+                    mine &= i >= j;
+                    p += exp(z.data[i] / t - g.lt);
+                }
+            if (!mine) continue;
+        }
+        const float xv = to_float(x.base[u + (long long)a0 * N]);
+        const double q = exp(((double)xv - g.ref) / t) * g.qf;
+        out[u + (long long)a0 * N] = from_float<T>(g.P == 0.0 ? 0.f : (float)(g.w / t * (g.P * q - p)));
+    }
+}
+
+// The other rows.
+template <typename T, int THREADS>
+__device__ __forceinline__ void write_rows(const Column<T> &x, T *out, int a0, int a1, const Slope &g, const unsigned *marks) {
     constexpr int N = Pack<T>::N;
     constexpr int U = 4;
     const int tid = threadIdx.x;
-    T *out = dx - x.shift;                                  // position u is out[u]
     const bool wide = ((reinterpret_cast<uintptr_t>(out)) & 15) == 0;
-    for (int a0 = v0; a0 < v1; a0 += kMarkRows / N) {
-        const int a1 = min(v1, a0 + kMarkRows / N);
-        const long long u0 = (long long)a0 * N, u1 = (long long)a1 * N;
-        __syncthreads();
-        for (int i = tid; i < kMarkRows / 32; i += THREADS) marks[i] = 0;
-        __syncthreads();
-        bool twice = false;
-        for (int j = e.j0 + tid; j < e.j1; j += THREADS) {
-            const int row = z.ir[j];
-            const long long u = (long long)row + x.shift - u0;
-            if (row < 0 || row >= x.rows || u < 0 || u >= u1 - u0) continue;
-            twice |= (atomicOr(&marks[u >> 5], 1u << (u & 31)) >> (u & 31)) & 1u;
+    const unsigned long long mr = pair(-g.ref, -g.ref), cc = pair(g.c, g.c), ff = pair(g.f, g.f);
+    auto scaled = [&](const uint4 &r) {
+        float v[N];
+        Pack<T>::unpack(r, v);
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
+            const float2 y = unpair(mul2(pair(q.x, q.y), ff));
+            v[j] = y.x;
+            v[j + 1] = y.y;
         }
-        twice = __syncthreads_or(twice);
-        for (int j = e.j0 + tid; j < e.j1; j += THREADS) {
-            const int row = z.ir[j];
-            const long long u = (long long)row + x.shift - u0;
-            if (row < 0 || row >= x.rows || u < 0 || u >= u1 - u0) continue;
-            double p = exp(z.data[j] / t - e.lt);
-            bool mine = true;
-            if (twice) {                                    // a row's first entry adds them up in their order
-                p = 0.0;
-                for (int i = e.j0; i < e.j1; i++)
-                    if (z.ir[i] == row) {
-                        mine &= i >= j;
-                        p += exp(z.data[i] / t - e.lt);
-                    }
-            }
-            if (mine) {
-                const double q = exp(((double)to_float(x.base[u + u0]) - ref) / t) * qf;
-                out[u + u0] = from_float<T>((float)(w / t * (e.P * q - p)));
-            }
+        return Pack<T>::pack(v);
+    };
+    // what of vector i is neither marked nor in `skip`
+    auto store = [&](int i, const uint4 &y, unsigned skip) {
+        const int b = (i - a0) * N;
+        skip |= (marks[b >> 5] >> (b & 31)) & ((1u << N) - 1u);
+        if (wide && !skip) {
+            store16(out + (long long)i * N, y);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (!((skip >> j) & 1u)) out[(long long)i * N + j] = reinterpret_cast<const T *>(&y)[j];
         }
-        auto scaled = [&](const uint4 &r) {
-            const unsigned long long mr = pair(-ref, -ref), cc = pair(c, c), ff = pair(f, f);
-            float v[N];
-            Pack<T>::unpack(r, v);
+    };
+    const int f1 = min(a1, x.full1);
+    int i = max(a0, x.full0) + tid;
+    for (; i < f1 - (U - 1) * THREADS; i += U * THREADS) {
+        uint4 r[U];
 #pragma unroll
-            for (int j = 0; j < N; j += 2) {
-                const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
-                const float2 y = unpair(mul2(pair(q.x, q.y), ff));
-                v[j] = y.x;
-                v[j + 1] = y.y;
-            }
-            return Pack<T>::pack(v);
-        };
-        // what of vector i is neither marked nor `skip`
-        auto store = [&](int i, const uint4 &y, unsigned skip) {
-            const int b = (i - a0) * N;
-            skip |= (marks[b >> 5] >> (b & 31)) & ((1u << N) - 1u);
-            if (wide && !skip) {
-                store16(out + (long long)i * N, y);
-            } else {
+        for (int k = 0; k < U; k++) r[k] = x.load(i + k * THREADS);
 #pragma unroll
-                for (int j = 0; j < N; j++)
-                    if (!((skip >> j) & 1u)) out[(long long)i * N + j] = reinterpret_cast<const T *>(&y)[j];
-            }
-        };
-        const int f1 = min(a1, x.full1);
-        int i = max(a0, x.full0) + tid;
-        for (; i < f1 - (U - 1) * THREADS; i += U * THREADS) {
-            uint4 r[U];
-#pragma unroll
-            for (int k = 0; k < U; k++) r[k] = x.load(i + k * THREADS);
-#pragma unroll
-            for (int k = 0; k < U; k++) store(i + k * THREADS, scaled(r[k]), 0);
-        }
-        for (; i < f1; i += THREADS) store(i, scaled(x.load(i)), 0);
-        if (tid < 2) {
-            const int p = x.partial(tid, a0, a1);
-            if (p >= 0) {
-                unsigned skip = 0;
-                for (int j = 0; j < N; j++) skip |= x.inside(p, j) ? 0u : 1u << j;
-                store(p, scaled(x.load_partial(p)), skip);
-            }
+        for (int k = 0; k < U; k++) store(i + k * THREADS, scaled(r[k]), 0);
+    }
+    for (; i < f1; i += THREADS) store(i, scaled(x.load(i)), 0);
+    if (tid < 2) {
+        const int p = x.partial(tid, a0, a1);
+        if (p >= 0) {
+            unsigned skip = 0;
+            for (int j = 0; j < N; j++) skip |= x.inside(p, j) ? 0u : 1u << j;
+            store(p, scaled(x.load_partial(p)), skip);
         }
     }
 }
 
+// The vectors [v0, v1) of the gradient, read again, stretch by stretch.
 template <typename T, int THREADS>
-__device__ __forceinline__ void write_zeros(const Column<T> &x, T *dx, int v0, int v1) {
+__device__ __forceinline__ void write_gradient(const Column<T> &x, T *out, const Teacher &z, int j0, int j1, int v0, int v1,
+                                               const Slope &g, unsigned *marks, int *twice) {
+    for (int a0 = v0; a0 < v1; a0 += kMarkRows / Pack<T>::N) {
+        const int a1 = min(v1, a0 + kMarkRows / Pack<T>::N);
+        __syncthreads();
+        if (threadIdx.x < kStream) mark_entries<T, kStream>(x, z, j0, j1, a0, a1, marks, twice);
+        __syncthreads();
+        write_entries<T>(x, out, z, j0, j1, a0, a1, g, *twice, (int)threadIdx.x, THREADS);
+        write_rows<T, THREADS>(x, out, a0, a1, g, marks);
+    }
+}
+
+template <typename T, int THREADS>
+__device__ __forceinline__ void write_zeros(const Column<T> &x, T *out, int v0, int v1) {
     constexpr int N = Pack<T>::N;
-    T *out = dx - x.shift;
     const bool wide = ((reinterpret_cast<uintptr_t>(out)) & 15) == 0;
     for (int i = v0 + (int)threadIdx.x; i < v1; i += THREADS) {
         if (wide && i >= x.full0 && i < x.full1) {
@@ -186,115 +268,348 @@ struct DistillArgs {
     float *loss, *lse_out;
 };
 
-// One cluster per column.  GRAD: also write the gradient, after the CTAs have joined their sums.
-template <typename T, bool GRAD>
-__global__ void __launch_bounds__(kThreadsAll, 4)
-distill_kernel(DistillArgs a, const T *X, T *dX) {
-    __shared__ float2 parts[kStream / 32];
-    __shared__ float2 joined[8];                   // (m, s) of every CTA of the cluster
-    __shared__ Entries entries;
-    __shared__ unsigned marks[GRAD ? kMarkRows / 32 : 1];
+// ---------------------------------------------------------------- columns that fit shared memory
+//
+// A CTA has a part of a column, which starts on its way to shared memory as the first thing.  Meanwhile one more warp
+// goes through the entries: a chain of dependent loads and fp64 exponentials that takes about as long.  It marks the
+// entries' rows, which the other warps leave out when they write, and writes those itself.
+//   BOTH: the CTAs of a cluster have one column.  Every warp sums up its rows and sends (m, s) to every CTA.
+//   GRAD: the log-sum-exp is given; CTAs have nothing to do with one another.
+// CTAs are short-lived and five of them share an SM, so that one's loads overlap another's arithmetic and stores.
+enum Mode { GRAD, BOTH };
+
+// What the columns have in common: a column's vectors start `shift` elements before it.
+struct Layout {
+    int ncols, parts, per;          // parts of a column, vectors per part
+    int shift0, ldmod;              // shift of column 0; how it moves from column to column
+};
+// A part of a column: vectors base[0 .. n), the first of them number v0 of the column.
+template <typename T> struct Slice {
+    static constexpr int N = Pack<T>::N;
+    const T *base;
+    int v0, n, shift;
+    int head, tail;                 // positions of vector 0 and of vector `last` that are not the column's
+    int last;                       // the column's last vector, relative to v0
+    __device__ __forceinline__ Slice(const T *X, long long ld, int rows, const Layout &l, int col, int part) {
+        shift = (l.shift0 + (col & (N - 1)) * l.ldmod) & (N - 1);
+        v0 = part * l.per;
+        const int nvec = (shift + rows + N - 1) / N;
+        n = max(min(nvec - v0, l.per), 0);
+        base = X + (col * ld + ((long long)v0 * N - shift));
+        head = v0 == 0 ? shift : 0;
+        last = nvec - 1 - v0;
+        tail = last >= 0 && last < n ? nvec * N - shift - rows : 0;
+    }
+    // vector 0, the last vector lie in the matrix that goes from X to end
+    __device__ __forceinline__ bool whole_head(const T *X) const { return base >= X; }
+    __device__ __forceinline__ bool whole_tail(const T *end) const { return base + ((long long)last + 1) * N <= end; }
+};
+
+// The sum of what every warp of the cluster has sent here.
+template <int W> __device__ __forceinline__ SumExp receive(unsigned long long *arrived, const float2 *joined, int count, float c) {
+    const bool ok = mail_wait(arrived, 0);
+    SumExp s;
+    for (int i = threadIdx.x & 31; i < count; i += 32) join(s, joined[i].x, joined[i].y, c);
+    warp_join(s, c);
+    if (!ok) s.s = NAN;             // never seen; an answer that cannot be mistaken for one
+    return s;
+}
+
+__device__ __forceinline__ void write_loss(const DistillArgs &a, long long col, const SumExp &s, const Entries &e, float w) {
+    const double L = s.m == -INFINITY ? (double)(s.s == 0.f ? -INFINITY : NAN) : s.m / (double)a.t + log((double)s.s);
+    if (a.lse_out) a.lse_out[col] = (float)L;
+    a.loss[col] = e.P == 0.0 ? 0.f : (float)((double)w * (e.cross + e.P * (L - e.lt)));
+}
+
+template <typename T, int THREADS, Mode MODE>
+__global__ void __launch_bounds__(THREADS + 32, THREADS == 256 ? 5 : 14)
+distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
+    constexpr int N = Pack<T>::N, W = THREADS / 32;
+    __shared__ float2 joined[MODE == GRAD ? 1 : 8 * W];         // (m, s) of every warp of the cluster
+    __shared__ unsigned long long arrived;
+    __shared__ float2 slope;                                    // factor P w/t, in GRAD times the rest of the reference; reference
+    __shared__ int twice;                                       // 1: a row came twice, 2: the gradient is zero
+    extern __shared__ uint4 kept[];                             // the part's vectors, then its marks: a byte per vector, a bit per element
+    unsigned char *marks = reinterpret_cast<unsigned char *>(kept + l.per);
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, rank = (int)cluster.block_rank(), size = (int)cluster.num_blocks();
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int col = (int)(blockIdx.x / (unsigned)l.parts), part = (int)(blockIdx.x % (unsigned)l.parts);
+    const Slice<T> x(X, a.ldx, a.nrows, l, col, part);
+    const int j0 = max(a.z.jc[col], 0), j1 = min(a.z.jc[col + 1], a.z.nnz);
+    const float w = a.weights ? a.weights[col] : 1.f;
+    const float lse = MODE == GRAD ? a.lse_in[col] : 0.f;
+    const T *const end = X + (l.ncols - 1) * a.ldx + a.nrows;
+    T *out = dX + (col * a.lddx + ((long long)x.v0 * N - x.shift));     // position 0 of the part
+
+    if (w == 0.f || j1 <= j0) {         // nothing is read; the whole cluster goes this way
+        const Column<T> whole(X + col * a.ldx, a.nrows);
+        write_zeros<T, THREADS + 32>(whole, dX + col * a.lddx - x.shift, x.v0, x.v0 + x.n);
+        if (MODE == BOTH && part == 0 && tid == 0) a.loss[col] = 0.f;
+        return;
+    }
+    // copies: partial vectors whole where their neighbours belong to the matrix as well
+    const int lo = x.head && !x.whole_head(X), hi = x.n - (x.tail && !x.whole_tail(end));
+    if (tid < THREADS) {
+        const T *p = x.base + (long long)tid * N;
+#pragma unroll 4
+        for (int i = tid; i < hi; i += THREADS, p += THREADS * N)
+            if (i >= lo) copy16(kept + i, p);
+    }
+    if (MODE == BOTH) {
+        if (tid == 0) {
+            mail_init(&arrived);
+            mail_init_done();
+            mail_expect(&arrived, l.parts * W * 8);
+        }
+        cluster_arrive();               // every CTA has its barrier before anything is sent to it
+    }
+    if (tid >= THREADS) {
+        Held h;
+        float xr[R], pr[R];
+        hold(h, a.z, j0, j1);
+        for (int i = lane; i < (l.per + 15) / 16; i += 32) reinterpret_cast<uint4 *>(marks)[i] = make_uint4(0, 0, 0, 0);
+        if (lane == 0) twice = 0;
+        __syncwarp();
+        auto mark = [&](int u) {                                // a position of the part
+            const int byte = u / N, bit = (byte & 3) * 8 + (u & (N - 1));
+            return (atomicOr(reinterpret_cast<unsigned *>(marks) + (byte >> 2), 1u << bit) >> bit) & 1u;
+        };
+        auto mark_row = [&](int r) {
+            const int u = r + x.shift - x.v0 * N;
+            if (r >= 0 && r < a.nrows && u >= 0 && u < x.n * N && mark(u)) atomicOr(&twice, 1);
+        };
+        if (lane < x.head) mark(lane);
+        if (lane < x.tail) mark(x.last * N + N - 1 - lane);
+#pragma unroll
+        for (int r = 0; r < R; r++) mark_row(h.row[r]);
+        for (int j = j0 + 32 * R + lane; j < j1; j += 32) mark_row(a.z.ir[j]);
+        // only CTA 0 needs the student's logits of all entries, for the loss
+        Entries e = MODE == BOTH && part == 0 ? weigh_entries<T, true>(h, a.z, col, a.nrows, a.t, X + col * a.ldx, xr, pr)
+                                              : weigh_entries<T, false>(h, a.z, col, a.nrows, a.t, nullptr, xr, pr);
+        float ref = 0.f, qf = 1.f;
+        if (MODE == GRAD) {
+            ref = (float)((double)lse * a.t);
+            qf = (float)exp(ref / (double)a.t - lse);           // what the rounding of the reference leaves
+        }
+        if (lane == 0) {
+            slope = make_float2((float)e.P * w / a.t * qf, ref);
+            if (e.P == 0.0) atomicOr(&twice, 2);
+        }
+        if (MODE == BOTH) cluster_wait();
+        __syncthreads();                                        // marks, slope; the part is in shared memory
+        if (MODE == BOTH) {
+            const SumExp s = receive<W>(&arrived, joined, l.parts * W, a.c);
+            ref = s.ref();
+            qf = 1.f / s.s;
+            if (part == 0 && lane == 0) write_loss(a, col, s, e, w);
+        }
+        const bool plain = (twice & 1) == 0;
+        if (plain) {
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                const int u = h.row[r] + x.shift - x.v0 * N;
+                if (h.row[r] >= 0 && h.row[r] < a.nrows && u >= 0 && u < x.n * N) {
+                    const float q = exp2_fast((to_float(reinterpret_cast<const T *>(kept)[u]) - ref) * a.c) * qf;
+                    out[u] = from_float<T>(e.P == 0.0 ? 0.f : w / a.t * ((float)e.P * q - pr[r]));
+                }
+            }
+        }
+        if (!plain || j1 - j0 > 32 * R) {
+            const Slope g{a.t, a.c, w, ref, 0.f, (double)qf, e.lt, e.P};
+            const Column<T> whole(X + col * a.ldx, a.nrows);
+            write_entries<T>(whole, dX + col * a.lddx - x.shift, a.z, plain ? j0 + 32 * R : j0, j1, x.v0, x.v0 + x.n, g, !plain, lane, 32);
+        }
+        return;
+    }
+
+    copies_commit();
+    copies_wait<0>();
+    if ((x.head && tid == 0) || (x.tail && tid == (x.last & (THREADS - 1)))) {
+        // partial vectors, by the threads they belong to: -infinity where they are not the column's
+        const Column<T> whole(X + col * a.ldx, a.nrows);
+        const bool one = x.head && x.tail && x.last == 0;
+        if (x.head && tid == 0)
+            kept[0] = x.whole_head(X) && !(one && !x.whole_tail(end)) ? whole.only_inside(0, kept[0]) : whole.load_partial(0);
+        if (x.tail && tid == (x.last & (THREADS - 1)) && !one)
+            kept[x.last] = x.whole_tail(end) ? whole.only_inside(x.last + x.v0, kept[x.last]) : whole.load_partial(x.last + x.v0);
+    }
+    float f, ref;
+    if (MODE == BOTH) {
+        SumExp s;
+#pragma unroll 4
+        for (int i = tid; i < x.n; i += THREADS) s.m = fmaxf(s.m, Pack<T>::max(kept[i]));
+        const unsigned long long mr = pair(-s.ref(), -s.ref()), cc = pair(a.c, a.c);
+        unsigned long long acc = pair(0.f, 0.f);
+#pragma unroll 2
+        for (int i = tid; i < x.n; i += THREADS) {
+            float v[N];
+            Pack<T>::unpack(kept[i], v);
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
+                acc = add2(acc, pair(q.x, q.y));
+            }
+        }
+        const float2 q = unpair(acc);
+        s.s = q.x + q.y;
+        warp_join(s, a.c);
+        cluster_wait();
+        if (lane < l.parts) mail_send(&joined[part * W + (tid >> 5)], &arrived, lane, make_float2(s.m, s.s));
+        __syncthreads();
+        const SumExp sum = receive<W>(&arrived, joined, l.parts * W, a.c);
+        ref = sum.ref();
+        f = slope.x / sum.s;
+    } else {
+        __syncthreads();
+        f = slope.x;
+        ref = slope.y;
+    }
+    const bool zero = (twice & 2) != 0, wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
+    const unsigned long long mr = pair(-ref, -ref), cc = pair(a.c, a.c), ff = pair(f, f);
+#pragma unroll 2
+    for (int i = tid; i < x.n; i += THREADS) {
+        float v[N];
+        Pack<T>::unpack(kept[i], v);
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
+            const float2 y = unpair(mul2(pair(q.x, q.y), ff));
+            v[j] = y.x;
+            v[j + 1] = y.y;
+        }
+        uint4 y = Pack<T>::pack(v);
+        if (zero) y = make_uint4(0, 0, 0, 0);
+        const unsigned skip = marks[i];
+        if (wide && !skip) {
+            store16(out + (long long)i * N, y);
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (!((skip >> j) & 1u)) out[(long long)i * N + j] = reinterpret_cast<const T *>(&y)[j];
+        }
+    }
+}
+
+// ---------------------------------------------------------------- columns of any length
+//
+// One cluster per column, also for the loss alone; the column is read twice for the gradient.  The last warp of CTA 0
+// looks after the entries, the others sum up their rows, and every warp leaves its sum with every CTA, or with CTA 0.
+template <typename T, bool GRADIENT>
+__global__ void __launch_bounds__(kStream + 32, GRADIENT ? 4 : 6)
+distill_long_kernel(DistillArgs a, const T *X, T *dX) {
+    constexpr int W = kStream / 32;
+    __shared__ float2 joined[8 * W];               // (m, s) of every warp of the cluster
+    __shared__ Entries entries;
+    __shared__ unsigned marks[GRADIENT ? kMarkRows / 32 + 1 : 1];
+    __shared__ int twice;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, rank = (int)cluster.block_rank(), size = (int)cluster.num_blocks();
     const long long col = blockIdx.x / size;
-    const double t = a.t;
     const Column<T> x(X + col * a.ldx, a.nrows);
     int v0, v1;
     my_part(x.nvec, rank, size, &v0, &v1);
-    const float w = a.weights ? a.weights[col] : 1.f;
+    T *out = GRADIENT ? dX + col * a.lddx - x.shift : nullptr;           // position u is out[u]
+    const float w = GRADIENT && a.weights ? a.weights[col] : 1.f;
     const int j0 = max(a.z.jc[col], 0), j1 = min(a.z.jc[col + 1], a.z.nnz);
-    if (GRAD && (w == 0.f || j1 <= j0)) {          // the whole cluster goes this way
-        write_zeros<T, kThreadsAll>(x, dX + col * a.lddx, v0, v1);
+    if (GRADIENT && (w == 0.f || j1 <= j0)) {          // the whole cluster goes this way
+        write_zeros<T, kStream + 32>(x, out, v0, v1);
         if (rank == 0 && tid == 0) a.loss[col] = 0.f;
         return;
     }
     cluster_arrive();                              // waited for before the first access to another CTA's memory
     if (tid >= kStream) {
+        Entries e;
         if (rank == 0) {
-            const Entries e = read_entries<T>(a.z, j0, j1, col, a.nrows, t, X + col * a.ldx);
-            if (tid == kStream) entries = e;
+            Held h;
+            float xr[R], pr[R];
+            hold(h, a.z, j0, j1);
+            e = weigh_entries<T, true>(h, a.z, col, a.nrows, a.t, X + col * a.ldx, xr, pr);
         }
+        cluster_wait();
+        if (rank == 0 && lane < (GRADIENT ? size : 1)) *cluster.map_shared_rank(&entries, lane) = e;
     } else {
-        SumExp s = sum_exp_slice<T, kStream>(x, v0, v1, a.c);
+        SumExp s = sum_exp_slice<T, kStream, 4>(x, v0, v1, a.c);
         warp_join(s, a.c);
-        if ((tid & 31) == 0) parts[tid >> 5] = make_float2(s.m, s.s);
+        cluster_wait();
+        if (lane < (GRADIENT ? size : 1)) *cluster.map_shared_rank(&joined[rank * W + (tid >> 5)], lane) = make_float2(s.m, s.s);
     }
+    cluster_arrive();
+    if (!GRADIENT && (rank != 0 || tid >= 32)) return;
     cluster_wait();
-    __syncthreads();
-    if (tid == 0) {
-        SumExp s;
-        for (int i = 0; i < kStream / 32; i++) join(s, parts[i].x, parts[i].y, a.c);
-        for (int r = 0; r < size; r++)
-            if (GRAD || r == 0) *cluster.map_shared_rank(&joined[rank], r) = make_float2(s.m, s.s);
-    }
-    if (GRAD && rank == 0 && tid > 0 && tid < size) *cluster.map_shared_rank(&entries, tid) = entries;
-    cluster.sync();
-    if (!GRAD && (rank != 0 || tid != 0)) return;
     SumExp s;
-    for (int r = 0; r < size; r++) join(s, joined[r].x, joined[r].y, a.c);
-    const Entries e = entries;
-    if (rank == 0 && tid == 0) {
-        const double L = s.m == -INFINITY ? (double)(s.s == 0.f ? -INFINITY : NAN) : s.m / t + log((double)s.s);
-        if (a.lse_out) a.lse_out[col] = (float)L;
-        a.loss[col] = e.P == 0.0 ? 0.f : (float)((GRAD ? (double)w : 1.0) * (e.cross + e.P * (L - e.lt)));
-    }
-    if (GRAD) {
+    for (int i = lane; i < size * W; i += 32) join(s, joined[i].x, joined[i].y, a.c);
+    warp_join(s, a.c);
+    const Entries &e = entries;
+    if (rank == 0 && tid == 0) write_loss(a, col, s, e, w);
+    if (GRADIENT) {
         if (e.P == 0.0) {
-            write_zeros<T, kThreadsAll>(x, dX + col * a.lddx, v0, v1);
-        } else {
-            const double qf = 1.0 / (double)s.s;
-            write_gradient<T, kThreadsAll>(x, dX + col * a.lddx, a.z, e, v0, v1, t, w, s.ref(), qf, (float)(e.P * w / t * qf), a.c, marks);
+            write_zeros<T, kStream + 32>(x, out, v0, v1);
+            return;
         }
+        const Slope g{a.t, a.c, w, s.ref(), (float)e.P * w / (a.t * s.s), 1.0 / s.s, e.lt, e.P};
+        write_gradient<T, kStream + 32>(x, out, a.z, j0, j1, v0, v1, g, marks, &twice);
     }
 }
 
-// The gradient from a saved log-sum-exp: `size` CTAs per column, each on its own.
-template <typename T>
-__global__ void __launch_bounds__(kStream, 5)
-distill_grad_kernel(DistillArgs a, int size, const T *X, T *dX) {
-    __shared__ Entries entries;
-    __shared__ unsigned marks[kMarkRows / 32];
-    const int tid = threadIdx.x, rank = (int)(blockIdx.x % size);
-    const long long col = blockIdx.x / size;
-    const double t = a.t;
-    const Column<T> x(X + col * a.ldx, a.nrows);
-    int v0, v1;
-    my_part(x.nvec, rank, size, &v0, &v1);
-    const float w = a.weights ? a.weights[col] : 1.f;
-    const int j0 = max(a.z.jc[col], 0), j1 = min(a.z.jc[col + 1], a.z.nnz);
-    bool none = w == 0.f || j1 <= j0;
-    if (!none) {
-        if (tid < 32) {
-            const Entries e = read_entries<T>(a.z, j0, j1, col, a.nrows, t, nullptr);
-            if (tid == 0) entries = e;
-        }
-        __syncthreads();
-        none = entries.P == 0.0;
-    }
-    if (none) {
-        write_zeros<T, kStream>(x, dX + col * a.lddx, v0, v1);
-        return;
-    }
-    const Entries e = entries;
-    const double L = a.lse_in[col];
-    const float ref = (float)(L * t);
-    const double qf = exp(ref / t - L);
-    write_gradient<T, kStream>(x, dX + col * a.lddx, a.z, e, v0, v1, t, w, ref, qf, (float)(e.P * w / t * qf), a.c, marks);
+// ---------------------------------------------------------------- host side
+
+// Vectors of the longest column, for the addresses that the columns really have.
+template <typename T> long long most_vectors(const void *X, long long ldx, int nrows, int ncols) {
+    constexpr int N = Pack<T>::N;
+    const bool even = is16(X) && (ncols == 1 || ldx % N == 0);
+    return ((long long)nrows + (even ? N - 1 : 2 * N - 2)) / N;
 }
 
-// CTAs of a cluster per column: enough of them to fill the machine (4 per SM), each with at least 8 KB.
-int cluster_for(int ncols, int nrows, int dtype, bool grad) {
-    const long long bytes = (long long)nrows * (long long)dtype_size(dtype);
-    int size = 1;
-    while (size < 8 && bytes / (2 * size) >= 8192 && ((long long)ncols * size < 592 || (grad && bytes / size > 65536))) size *= 2;
-    return size;
-}
-
-template <typename T, bool GRAD>
-cudaError_t launch_distill(const DistillArgs &a, int ncols, int size, const void *X, void *dX, cudaStream_t st) {
+template <typename T, int THREADS, Mode MODE>
+cudaError_t launch_part(const DistillArgs &a, int ncols, int parts, long long nvec, const void *X, void *dX, cudaStream_t st) {
+    constexpr int N = Pack<T>::N;
+    const auto kernel = distill_part_kernel<T, THREADS, MODE>;
+    const long long per = ((nvec + parts - 1) / parts + 7) & ~7LL;         // whole 128-byte lines
+    const size_t smem = (size_t)per * 16 + (((size_t)per + 15) & ~size_t(15));
+    if (smem > 40000) {
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return err;
+    }
+    if ((long long)ncols * parts > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)ncols * (unsigned)size, kThreadsAll, size, 0, st);
-    return cudaLaunchKernelEx(&cfg, distill_kernel<T, GRAD>, a, (const T *)X, (T *)dX);
+    const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)(ncols * parts), THREADS + 32, MODE == GRAD ? 1 : parts, smem, st);
+    const Layout l{ncols, parts, (int)per, (int)((reinterpret_cast<uintptr_t>(X) & 15) / sizeof(T)), (int)(a.ldx & (N - 1))};
+    return cudaLaunchKernelEx(&cfg, kernel, a, l, (const T *)X, (T *)dX);
+}
+
+template <typename T, bool GRADIENT>
+cudaError_t launch_long(const DistillArgs &a, int ncols, int size, const void *X, void *dX, cudaStream_t st) {
+    if ((long long)ncols * size > 0x7fffffffLL) return cudaErrorInvalidValue;
+    cudaLaunchAttribute attr;
+    const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)(ncols * size), kStream + 32, size, 0, st);
+    return cudaLaunchKernelEx(&cfg, distill_long_kernel<T, GRADIENT>, a, (const T *)X, (T *)dX);
+}
+
+// Parts of 32 KB keep five CTAs on an SM; a cluster has at most 8 parts, so columns of up to 512 KB get larger ones, and
+// those beyond are read twice.  Where columns are few they are cut into more parts, to give every SM two CTAs.  Columns of
+// up to 8 KB have a small CTA each.
+constexpr long long kPartBytes = 32768, kMostPartBytes = 65536, kShortBytes = 8192;
+
+template <typename T, Mode MODE>
+cudaError_t launch_distill(const DistillArgs &a, int ncols, const void *X, void *dX, cudaStream_t st) {
+    const long long nvec = most_vectors<T>(X, a.ldx, a.nrows, ncols), bytes = nvec * 16;
+    const long long most = MODE == GRAD ? nvec : 8;
+    const bool small = bytes <= kShortBytes;
+    long long parts = (bytes + kPartBytes - 1) / kPartBytes;
+    const long long fill = (296 + ncols - 1) / ncols, worth = (nvec + (small ? 63 : 255)) / (small ? 64 : 256);
+    if (parts < fill) parts = fill < worth ? fill : worth;
+    if (parts > most) parts = most;
+    if (small) return launch_part<T, 64, MODE>(a, ncols, (int)parts, nvec, X, dX, st);
+    if (bytes <= parts * kMostPartBytes) return launch_part<T, 256, MODE>(a, ncols, (int)parts, nvec, X, dX, st);
+    return launch_long<T, true>(a, ncols, 8, X, dX, st);
+}
+
+// Without a gradient nothing has to stay on the chip, and a CTA is best kept on one column as long as there are
+// enough of them (131072 x 2048 bf16: 89 us in one part, 106 us in two, 126 us in four).
+template <typename T> cudaError_t launch_loss(const DistillArgs &a, int ncols, const void *X, cudaStream_t st) {
+    const long long bytes = (long long)a.nrows * (long long)sizeof(T);
+    const long long fill = (592 + ncols - 1) / ncols, worth = (bytes + 8191) / 8192, parts = fill < worth ? fill : worth;
+    return launch_long<T, false>(a, ncols, (int)(parts < 8 ? parts : 8), X, nullptr, st);
 }
 
 DistillArgs arguments(int nrows, long long ldx, long long lddx, float t, const Teacher &z, const float *weights, const float *lse_in,
@@ -304,7 +619,7 @@ DistillArgs arguments(int nrows, long long ldx, long long lddx, float t, const T
 
 int check(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype, float temperature, const int *Zir,
           const int *Zjc, const float *Zdata) {
-    if (nrows < 1 || ncols < 0 || nnz < 0 || !dtype_ok(dtype)) return (int)cudaErrorInvalidValue;
+    if (nrows < 1 || nrows > kMostRows || ncols < 0 || ncols > kMostRows || nnz < 0 || !dtype_ok(dtype)) return (int)cudaErrorInvalidValue;
     if (!isfinite(temperature) || temperature <= 0.f) return (int)cudaErrorInvalidValue;
     if (ncols == 0) return 0;
     if (!dense_ok(X, ldx, nrows, dtype) || !Zjc || (nnz > 0 && (!Zir || !Zdata))) return (int)cudaErrorInvalidValue;
@@ -321,10 +636,8 @@ extern "C" int bidmat_b200_distill(int nrows, int ncols, int nnz, const void *X,
     if (ncols == 0) return 0;
     if (!loss || !Xlse) return (int)cudaErrorInvalidValue;
     const DistillArgs a = arguments(nrows, ldx, 0, temperature, Teacher{Zir, Zjc, Zdata, Zlse, nnz}, nullptr, nullptr, loss, Xlse);
-    const int size = cluster_for(ncols, nrows, dtype, false);
-    if ((long long)ncols * size > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     cudaError_t err = cudaSuccess;
-#define CALL_LOSS(T) err = launch_distill<T, false>(a, ncols, size, X, nullptr, as_stream(stream))
+#define CALL_LOSS(T) err = launch_loss<T>(a, ncols, X, as_stream(stream))
     DISPATCH_DTYPE(dtype, CALL_LOSS);
 #undef CALL_LOSS
     g_launches += 1;
@@ -341,19 +654,12 @@ extern "C" int bidmat_b200_distill_grad(int nrows, int ncols, int nnz, const voi
     if (!Xlse || !dense_ok(dX, lddx, nrows, dtype)) return (int)cudaErrorInvalidValue;
     if (X == dX && ldx != lddx) return (int)cudaErrorInvalidValue;
     const DistillArgs a = arguments(nrows, ldx, lddx, temperature, Teacher{Zir, Zjc, Zdata, Zlse, nnz}, weights, Xlse, nullptr, nullptr);
-    // CTAs per column: eight per SM in all, stretches of 2048 rows or more, one stretch of marks at most where that gives enough
-    long long size = ((long long)nrows + kMarkRows - 1) / kMarkRows;
-    const long long fill = (1184 + (long long)ncols - 1) / ncols;
-    if (size < fill) size = fill;
-    const long long most = ((long long)nrows + 2047) / 2048;
-    if (size > most) size = most;
-    if (size * ncols > 0x7fffffffLL) size = 0x7fffffffLL / ncols;
-    cudaStream_t st = as_stream(stream);
-#define CALL_GRAD(T)                                                                                                     distill_grad_kernel<T><<<(unsigned)(size * ncols), kStream, 0, st>>>(a, (int)size, (const T *)X, (T *)dX)
+    cudaError_t err = cudaSuccess;
+#define CALL_GRAD(T) err = launch_distill<T, GRAD>(a, ncols, X, dX, as_stream(stream))
     DISPATCH_DTYPE(dtype, CALL_GRAD);
 #undef CALL_GRAD
     g_launches += 1;
-    return (int)cudaGetLastError();
+    return (int)err;
 }
 
 extern "C" int bidmat_b200_distill_with_grad(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
@@ -366,10 +672,8 @@ extern "C" int bidmat_b200_distill_with_grad(int nrows, int ncols, int nnz, cons
     if (!loss || !dense_ok(dX, lddx, nrows, dtype)) return (int)cudaErrorInvalidValue;
     if (X == dX && ldx != lddx) return (int)cudaErrorInvalidValue;
     const DistillArgs a = arguments(nrows, ldx, lddx, temperature, Teacher{Zir, Zjc, Zdata, Zlse, nnz}, weights, nullptr, loss, nullptr);
-    const int size = cluster_for(ncols, nrows, dtype, true);
-    if ((long long)ncols * size > 0x7fffffffLL) return (int)cudaErrorInvalidValue;
     cudaError_t err = cudaSuccess;
-#define CALL_BOTH(T) err = launch_distill<T, true>(a, ncols, size, X, dX, as_stream(stream))
+#define CALL_BOTH(T) err = launch_distill<T, BOTH>(a, ncols, X, dX, as_stream(stream))
     DISPATCH_DTYPE(dtype, CALL_BOTH);
 #undef CALL_BOTH
     g_launches += 1;

@@ -24,10 +24,11 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// N elements of one 16-byte vector as floats and back.
+// N elements of one 16-byte vector as floats and back; lowest: all -infinity.
 template <typename T> struct Pack;
 template <> struct Pack<float> {
     static constexpr int N = 4;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
     }
@@ -37,9 +38,16 @@ template <> struct Pack<float> {
     static __device__ __forceinline__ float max(const uint4 &r) {
         return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
     }
+    template <int K> static __device__ __forceinline__ float max_of(const uint4 (&r)[K]) {
+        float m = max(r[0]);
+#pragma unroll
+        for (int k = 1; k < K; k++) m = fmaxf(m, max(r[k]));
+        return m;
+    }
 };
 template <> struct Pack<__nv_bfloat16> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         const unsigned w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -62,9 +70,17 @@ template <> struct Pack<__nv_bfloat16> {
         const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
         return fmaxf(__low2float(m), __high2float(m));
     }
+    template <int K> static __device__ __forceinline__ float max_of(const uint4 (&r)[K]) {
+        const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(r);
+        __nv_bfloat162 m = p[0];
+#pragma unroll
+        for (int k = 1; k < 4 * K; k++) m = __hmax2(m, p[k]);
+        return fmaxf(__low2float(m), __high2float(m));
+    }
 };
 template <> struct Pack<__half> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         const __half2 *p = reinterpret_cast<const __half2 *>(&r);
 #pragma unroll
@@ -86,6 +102,13 @@ template <> struct Pack<__half> {
     static __device__ __forceinline__ float max(const uint4 &r) {
         const __half2 *p = reinterpret_cast<const __half2 *>(&r);
         const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
+        return fmaxf(__low2float(m), __high2float(m));
+    }
+    template <int K> static __device__ __forceinline__ float max_of(const uint4 (&r)[K]) {
+        const __half2 *p = reinterpret_cast<const __half2 *>(r);
+        __half2 m = p[0];
+#pragma unroll
+        for (int k = 1; k < 4 * K; k++) m = __hmax2(m, p[k]);
         return fmaxf(__low2float(m), __high2float(m));
     }
 };
@@ -129,6 +152,14 @@ template <typename T> struct Column {
         for (int j = 0; j < N; j++) v[j] = inside(i, j) ? to_float(base[(long long)i * N + j]) : -INFINITY;
         return Pack<T>::pack(v);
     }
+    // vector i with -infinity where it is not the column's
+    __device__ __forceinline__ uint4 only_inside(int i, const uint4 &r) const {
+        float v[N];
+        Pack<T>::unpack(r, v);
+#pragma unroll
+        for (int j = 0; j < N; j++) v[j] = inside(i, j) ? v[j] : -INFINITY;
+        return Pack<T>::pack(v);
+    }
     // The partial vectors among [v0, v1): number 0 and 1, or -1.
     __device__ __forceinline__ int partial(int number, int v0, int v1) const {
         const int i = number == 0 ? 0 : nvec - 1;
@@ -139,9 +170,52 @@ template <typename T> struct Column {
     }
 };
 
+// Asynchronous copies of 16 bytes to shared memory; their thread waits for all of its own.
+__device__ __forceinline__ void copy16(void *smem, const void *p) {
+    const unsigned dst = (unsigned)__cvta_generic_to_shared(smem);
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
+}
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+// All but the last PENDING groups have arrived.
+template <int PENDING> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
 // The two halves of a cluster-wide barrier.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
+// An arrival that orders no memory: the fence of the other form waits for every store before it.
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
+
+// A barrier in shared memory that counts arriving bytes, for values that other CTAs of the cluster send here.
+__device__ __forceinline__ unsigned smem_address(const void *p) { return (unsigned)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ void mail_init(unsigned long long *bar) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(smem_address(bar)) : "memory");
+}
+__device__ __forceinline__ void mail_init_done() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
+__device__ __forceinline__ void mail_expect(unsigned long long *bar, unsigned bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_address(bar)), "r"(bytes) : "memory");
+}
+// Two floats to the same place of CTA `rank`, whose barrier counts them when they are there.
+__device__ __forceinline__ void mail_send(float2 *to, unsigned long long *bar, int rank, float2 v) {
+    unsigned dst, b;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(dst) : "r"(smem_address(to)), "r"(rank));
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(b) : "r"(smem_address(bar)), "r"(rank));
+    asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1,%2}, [%3];" ::"r"(dst), "f"(v.x), "f"(v.y),
+                 "r"(b)
+                 : "memory");
+}
+// Waits for phase `parity`, with a limit of about a second; false when it ran out.
+__device__ __forceinline__ bool mail_wait(unsigned long long *bar, unsigned parity) {
+    const unsigned b = smem_address(bar);
+    for (int i = 0; i < (1 << 20); i++) {
+        unsigned ok;
+        asm volatile("{\n.reg .pred p;\nmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2, 1000;\nselp.u32 %0, 1, 0, p;\n}"
+                     : "=r"(ok)
+                     : "r"(b), "r"(parity)
+                     : "memory");
+        if (ok) return true;
+    }
+    return false;
+}
 
 struct SumExp {
     float m = -INFINITY, s = 0.f;
@@ -207,18 +281,23 @@ __device__ __forceinline__ void join(SumExp &a, float m, float s, float c) {
         a.s += s == 0.f ? 0.f : (m == a.m ? s : s * exp2_fast((m - a.m) * c));
     }
 }
+// Largest of the warp's values (none of them NaN).
+__device__ __forceinline__ float warp_top(float v) {
+    float r;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(r) : "f"(v));
+    return r;
+}
+// The same result in every lane: the sums are brought up to the largest maximum, then added.
 __device__ __forceinline__ void warp_join(SumExp &a, float c) {
-#pragma unroll
-    for (int o = 16; o; o >>= 1) {
-        const float m = __shfl_xor_sync(0xffffffffu, a.m, o), s = __shfl_xor_sync(0xffffffffu, a.s, o);
-        join(a, m, s, c);
-    }
+    const float m = warp_top(a.m);
+    a.s = a.m == m || a.s == 0.f ? a.s : a.s * exp2_fast((a.m - m) * c);
+    a.m = m;
+    a.s = warp_sum(a.s);
 }
 
-// The vectors [v0, v1) of a column, four loads in flight per thread.
-template <typename T, int THREADS>
+// The vectors [v0, v1) of a column, U loads in flight per thread.
+template <typename T, int THREADS, int U>
 __device__ __forceinline__ SumExp sum_exp_slice(const Column<T> &x, int v0, int v1, float c) {
-    constexpr int U = 4;
     SumExp a;
     const int f1 = min(v1, x.full1);
     int i = max(v0, x.full0) + (int)threadIdx.x;

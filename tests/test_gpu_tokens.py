@@ -261,7 +261,8 @@ def test_route_gradient_of_any_sparse_matrix(cuda_device):
 
 def lse_tolerance(x, L, tau):
     V = x.shape[1]
-    f = np.where(np.isfinite(x), x, 0.0)
+    # what is masked, be it by a value like the lowest of the type, has no part in the exponents' rounding
+    f = np.where(np.abs(x) < 1e30, x, 0.0)
     span = (f.max(1) - f.min(1)) / tau
     return U * (np.abs(np.where(np.isfinite(L), L, 0.0)) + 2 * span + V / 256.0 + 16)
 
@@ -367,7 +368,7 @@ def check_distill(x, jc, ir, z, dtype, device, tau=1.0, tlse=None, weights=None,
             r = ir[jc[t]:jc[t + 1]]
             ok = (r >= 0) & (r < V)
             p[t, r[ok]] = np.abs(w[t]) / tau32 * P[t]
-        f = np.abs(np.where(np.isfinite(xs), xs, 0)).max() / tau32
+        f = np.abs(np.where(np.abs(xs) < 1e30, xs, 0)).max() / tau32
         return np.nan_to_num((dense_part + p) * (rel[:, None] + 8 * U + U * f) + 4 * U * p + HALF[dtype] * np.abs(g)) \
             + TINY[dtype] * (1 + np.nan_to_num(np.abs(w) / tau32 * P)[:, None])
 
@@ -378,7 +379,7 @@ def check_distill(x, jc, ir, z, dtype, device, tau=1.0, tlse=None, weights=None,
     saved = host(L.t)[:, 0]
     g2 = oracle64.distill(xs, jc, ir, z, tau32, tlse, weights, slse=saved)[2]
     dX2 = tokens.distillGrad(X, Z, L, weights=row(weights, device), temperature=tau, lse=row(tlse, device))
-    close(host(dX2.t), g2, gtol(g2, np.full(T, 4 * U * (1 + np.nanmax(np.abs(np.where(np.isfinite(saved), saved, 0)))))), "gradient from the saved pass")
+    close(host(dX2.t), g2, gtol(g2, 4 * U * (1 + np.abs(np.where(np.isfinite(saved), saved, 0)))), "gradient from the saved pass")
     again = tokens.distillWithGrad(X, Z, weights=row(weights, device), temperature=tau, lse=row(tlse, device))
     assert same_bits(again[0].t, wl.t) and same_bits(again[1].t, dX.t)
     return X, Z, wl, dX
