@@ -278,33 +278,6 @@ struct DistillArgs {
 // CTAs are short-lived and five of them share an SM, so that one's loads overlap another's arithmetic and stores.
 enum Mode { GRAD, BOTH };
 
-// What the columns have in common: a column's vectors start `shift` elements before it.
-struct Layout {
-    int ncols, parts, per;          // parts of a column, vectors per part
-    int shift0, ldmod;              // shift of column 0; how it moves from column to column
-};
-// A part of a column: vectors base[0 .. n), the first of them number v0 of the column.
-template <typename T> struct Slice {
-    static constexpr int N = Pack<T>::N;
-    const T *base;
-    int v0, n, shift;
-    int head, tail;                 // positions of vector 0 and of vector `last` that are not the column's
-    int last;                       // the column's last vector, relative to v0
-    __device__ __forceinline__ Slice(const T *X, long long ld, int rows, const Layout &l, int col, int part) {
-        shift = (l.shift0 + (col & (N - 1)) * l.ldmod) & (N - 1);
-        v0 = part * l.per;
-        const int nvec = (shift + rows + N - 1) / N;
-        n = max(min(nvec - v0, l.per), 0);
-        base = X + (col * ld + ((long long)v0 * N - shift));
-        head = v0 == 0 ? shift : 0;
-        last = nvec - 1 - v0;
-        tail = last >= 0 && last < n ? nvec * N - shift - rows : 0;
-    }
-    // vector 0, the last vector lie in the matrix that goes from X to end
-    __device__ __forceinline__ bool whole_head(const T *X) const { return base >= X; }
-    __device__ __forceinline__ bool whole_tail(const T *end) const { return base + ((long long)last + 1) * N <= end; }
-};
-
 // The sum of what every warp of the cluster has sent here.
 template <int W> __device__ __forceinline__ SumExp receive(unsigned long long *arrived, const float2 *joined, int count, float c) {
     const bool ok = mail_wait(arrived, 0);
@@ -347,14 +320,7 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
         if (MODE == BOTH && part == 0 && tid == 0) a.loss[col] = 0.f;
         return;
     }
-    // copies: partial vectors whole where their neighbours belong to the matrix as well
-    const int lo = x.head && !x.whole_head(X), hi = x.n - (x.tail && !x.whole_tail(end));
-    if (tid < THREADS) {
-        const T *p = x.base + (long long)tid * N;
-#pragma unroll 4
-        for (int i = tid; i < hi; i += THREADS, p += THREADS * N)
-            if (i >= lo) copy16(kept + i, p);
-    }
+    if (tid < THREADS) x.template copy<THREADS>(kept, X, end);
     if (MODE == BOTH) {
         if (tid == 0) {
             mail_init(&arrived);
@@ -422,17 +388,7 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
         return;
     }
 
-    copies_commit();
-    copies_wait<0>();
-    if ((x.head && tid == 0) || (x.tail && tid == (x.last & (THREADS - 1)))) {
-        // partial vectors, by the threads they belong to: -infinity where they are not the column's
-        const Column<T> whole(X + col * a.ldx, a.nrows);
-        const bool one = x.head && x.tail && x.last == 0;
-        if (x.head && tid == 0)
-            kept[0] = x.whole_head(X) && !(one && !x.whole_tail(end)) ? whole.only_inside(0, kept[0]) : whole.load_partial(0);
-        if (x.tail && tid == (x.last & (THREADS - 1)) && !one)
-            kept[x.last] = x.whole_tail(end) ? whole.only_inside(x.last + x.v0, kept[x.last]) : whole.load_partial(x.last + x.v0);
-    }
+    x.template arrive<THREADS>(kept, X, end, X + col * a.ldx, a.nrows);
     float f, ref;
     if (MODE == BOTH) {
         SumExp s;
@@ -553,16 +509,8 @@ distill_long_kernel(DistillArgs a, const T *X, T *dX) {
 
 // ---------------------------------------------------------------- host side
 
-// Vectors of the longest column, for the addresses that the columns really have.
-template <typename T> long long most_vectors(const void *X, long long ldx, int nrows, int ncols) {
-    constexpr int N = Pack<T>::N;
-    const bool even = is16(X) && (ncols == 1 || ldx % N == 0);
-    return ((long long)nrows + (even ? N - 1 : 2 * N - 2)) / N;
-}
-
 template <typename T, int THREADS, Mode MODE>
 cudaError_t launch_part(const DistillArgs &a, int ncols, int parts, long long nvec, const void *X, void *dX, cudaStream_t st) {
-    constexpr int N = Pack<T>::N;
     const auto kernel = distill_part_kernel<T, THREADS, MODE>;
     const long long per = ((nvec + parts - 1) / parts + 7) & ~7LL;         // whole 128-byte lines
     const size_t smem = (size_t)per * 16 + (((size_t)per + 15) & ~size_t(15));
@@ -573,7 +521,7 @@ cudaError_t launch_part(const DistillArgs &a, int ncols, int parts, long long nv
     if ((long long)ncols * parts > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)(ncols * parts), THREADS + 32, MODE == GRAD ? 1 : parts, smem, st);
-    const Layout l{ncols, parts, (int)per, (int)((reinterpret_cast<uintptr_t>(X) & 15) / sizeof(T)), (int)(a.ldx & (N - 1))};
+    const Layout l = layout<T>(X, a.ldx, ncols, parts, per);
     return cudaLaunchKernelEx(&cfg, kernel, a, l, (const T *)X, (T *)dX);
 }
 

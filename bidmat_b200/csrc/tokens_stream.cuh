@@ -24,11 +24,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
     return y;
 }
 
-// N elements of one 16-byte vector as floats and back; lowest: all -infinity.
+// The larger one, NaN if either is.
+__device__ __forceinline__ float larger_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
+
+// N elements of one 16-byte vector as floats and back.  max leaves NaN out, max_nan is NaN if any element is.
 template <typename T> struct Pack;
 template <> struct Pack<float> {
     static constexpr int N = 4;
-    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
     }
@@ -38,16 +44,12 @@ template <> struct Pack<float> {
     static __device__ __forceinline__ float max(const uint4 &r) {
         return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
     }
-    template <int K> static __device__ __forceinline__ float max_of(const uint4 (&r)[K]) {
-        float m = max(r[0]);
-#pragma unroll
-        for (int k = 1; k < K; k++) m = fmaxf(m, max(r[k]));
-        return m;
+    static __device__ __forceinline__ float max_nan(const uint4 &r) {
+        return larger_nan(larger_nan(__uint_as_float(r.x), __uint_as_float(r.y)), larger_nan(__uint_as_float(r.z), __uint_as_float(r.w)));
     }
 };
 template <> struct Pack<__nv_bfloat16> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         const unsigned w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -70,17 +72,14 @@ template <> struct Pack<__nv_bfloat16> {
         const __nv_bfloat162 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
         return fmaxf(__low2float(m), __high2float(m));
     }
-    template <int K> static __device__ __forceinline__ float max_of(const uint4 (&r)[K]) {
-        const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(r);
-        __nv_bfloat162 m = p[0];
-#pragma unroll
-        for (int k = 1; k < 4 * K; k++) m = __hmax2(m, p[k]);
-        return fmaxf(__low2float(m), __high2float(m));
+    static __device__ __forceinline__ float max_nan(const uint4 &r) {
+        const __nv_bfloat162 *p = reinterpret_cast<const __nv_bfloat162 *>(&r);
+        const __nv_bfloat162 m = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+        return larger_nan(__low2float(m), __high2float(m));
     }
 };
 template <> struct Pack<__half> {
     static constexpr int N = 8;
-    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         const __half2 *p = reinterpret_cast<const __half2 *>(&r);
 #pragma unroll
@@ -104,12 +103,10 @@ template <> struct Pack<__half> {
         const __half2 m = __hmax2(__hmax2(p[0], p[1]), __hmax2(p[2], p[3]));
         return fmaxf(__low2float(m), __high2float(m));
     }
-    template <int K> static __device__ __forceinline__ float max_of(const uint4 (&r)[K]) {
-        const __half2 *p = reinterpret_cast<const __half2 *>(r);
-        __half2 m = p[0];
-#pragma unroll
-        for (int k = 1; k < 4 * K; k++) m = __hmax2(m, p[k]);
-        return fmaxf(__low2float(m), __high2float(m));
+    static __device__ __forceinline__ float max_nan(const uint4 &r) {
+        const __half2 *p = reinterpret_cast<const __half2 *>(&r);
+        const __half2 m = __hmax2_nan(__hmax2_nan(p[0], p[1]), __hmax2_nan(p[2], p[3]));
+        return larger_nan(__low2float(m), __high2float(m));
     }
 };
 
@@ -316,7 +313,68 @@ __device__ __forceinline__ SumExp sum_exp_slice(const Column<T> &x, int v0, int 
     return a;
 }
 
+// What the columns have in common: a column's vectors start `shift` elements before it.
+struct Layout {
+    int ncols, parts, per;          // parts of a column, vectors per part
+    int shift0, ldmod;              // shift of column 0; how it moves from column to column
+};
+// A part of a column: vectors base[0 .. n), the first of them number v0 of the column.
+template <typename T> struct Slice {
+    static constexpr int N = Pack<T>::N;
+    const T *base;
+    int v0, n, shift;
+    int head, tail;                 // positions of vector 0 and of vector `last` that are not the column's
+    int last;                       // the column's last vector, relative to v0
+    __device__ __forceinline__ Slice(const T *X, long long ld, int rows, const Layout &l, int col, int part) {
+        shift = (l.shift0 + (col & (N - 1)) * l.ldmod) & (N - 1);
+        v0 = part * l.per;
+        const int nvec = (shift + rows + N - 1) / N;
+        n = max(min(nvec - v0, l.per), 0);
+        base = X + (col * ld + ((long long)v0 * N - shift));
+        head = v0 == 0 ? shift : 0;
+        last = nvec - 1 - v0;
+        tail = last >= 0 && last < n ? nvec * N - shift - rows : 0;
+    }
+    // vector 0, the last vector lie in the matrix that goes from X to end
+    __device__ __forceinline__ bool whole_head(const T *X) const { return base >= X; }
+    __device__ __forceinline__ bool whole_tail(const T *end) const { return base + ((long long)last + 1) * N <= end; }
+    // Starts the copies of a thread's vectors (tid, tid + THREADS, ...) to shared memory.  Partial vectors are copied
+    // whole where their neighbours belong to the matrix as well.
+    template <int THREADS> __device__ __forceinline__ void copy(uint4 *kept, const T *X, const T *end) const {
+        const int tid = threadIdx.x, lo = head && !whole_head(X), hi = n - (tail && !whole_tail(end));
+        const T *p = base + (long long)tid * N;
+#pragma unroll 4
+        for (int i = tid; i < hi; i += THREADS, p += THREADS * N)
+            if (i >= lo) copy16(kept + i, p);
+        copies_commit();
+    }
+    // Waits for them; partial vectors get -infinity where they are not the column's.
+    template <int THREADS>
+    __device__ __forceinline__ void arrive(uint4 *kept, const T *X, const T *end, const T *column, int rows) const {
+        const int tid = threadIdx.x;
+        copies_wait<0>();
+        if ((head && tid == 0) || (tail && tid == (last & (THREADS - 1)))) {
+            const Column<T> whole(column, rows);
+            const bool one = head && tail && last == 0;
+            if (head && tid == 0)
+                kept[0] = whole_head(X) && !(one && !whole_tail(end)) ? whole.only_inside(0, kept[0]) : whole.load_partial(0);
+            if (tail && tid == (last & (THREADS - 1)) && !one)
+                kept[last] = whole_tail(end) ? whole.only_inside(last + v0, kept[last]) : whole.load_partial(last + v0);
+        }
+    }
+};
+
 // ------------------------------------------------------------------ host side
+// Vectors of the longest column, for the addresses that the columns really have.
+template <typename T> long long most_vectors(const void *X, long long ldx, int nrows, int ncols) {
+    constexpr int N = Pack<T>::N;
+    const bool even = is16(X) && (ncols == 1 || ldx % N == 0);
+    return ((long long)nrows + (even ? N - 1 : 2 * N - 2)) / N;
+}
+template <typename T> Layout layout(const void *X, long long ldx, int ncols, int parts, long long per) {
+    return Layout{ncols, parts, (int)per, (int)((reinterpret_cast<uintptr_t>(X) & 15) / sizeof(T)), (int)(ldx & (Pack<T>::N - 1))};
+}
+
 // Clusters of `size` CTAs along x.
 inline cudaLaunchConfig_t cluster_config(cudaLaunchAttribute *attr, unsigned grid, unsigned threads, int size, size_t smem,
                                          cudaStream_t st) {

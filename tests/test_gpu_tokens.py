@@ -287,7 +287,7 @@ def check_top(x, dtype, device, k, tau=1.0, pad=0):
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("V,T,k", [(1, 1, 1), (2, 3, 2), (31, 5, 31), (512, 4, 512), (513, 3, 512), (1000, 9, 17), (4096, 2, 100),
                                    (8191, 3, 64), (32768, 1, 40), (50001, 5, 128), (131072, 2, 512), (100003, 3, 1),
-                                   (300007, 2, 50)])
+                                   (300007, 2, 50), (500009, 1, 70)])
 def test_top_sizes_and_types(cuda_device, dtype, V, T, k):
     rng = np.random.default_rng(V + T)
     check_top(2.0 * rng.standard_normal((T, V)), dtype, cuda_device, k, pad=0)
@@ -295,7 +295,7 @@ def test_top_sizes_and_types(cuda_device, dtype, V, T, k):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16"])
-@pytest.mark.parametrize("V", [700, 40000, 140000])
+@pytest.mark.parametrize("V", [700, 40000, 140000, 520001])
 def test_top_of_columns_in_bad_orders(cuda_device, dtype, V):
     """Ascending, descending, constant, two values, one spike, masked, equal large values at the far end."""
     k = 100
