@@ -252,13 +252,6 @@ __device__ __forceinline__ void write_zeros(const Column<T> &x, T *out, int v0, 
     }
 }
 
-// The part of nvec vectors that CTA `rank` of `size` has: whole 128-byte lines but for the last.
-__device__ __forceinline__ void my_part(int nvec, int rank, int size, int *v0, int *v1) {
-    const int per = (((nvec + size - 1) / size) + 7) & ~7;
-    *v0 = (int)min((long long)nvec, (long long)rank * per);
-    *v1 = (int)min((long long)nvec, (long long)(rank + 1) * per);
-}
-
 struct DistillArgs {
     int nrows;
     long long ldx, lddx;

@@ -31,10 +31,11 @@ __device__ __forceinline__ float larger_nan(float a, float b) {
     return r;
 }
 
-// N elements of one 16-byte vector as floats and back.  max leaves NaN out, max_nan is NaN if any element is.
+// N elements of one 16-byte vector as floats and back; lowest: all -infinity.  max leaves NaN out, max_nan is NaN if any element is.
 template <typename T> struct Pack;
 template <> struct Pack<float> {
     static constexpr int N = 4;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff800000u, 0xff800000u, 0xff800000u, 0xff800000u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
     }
@@ -50,6 +51,7 @@ template <> struct Pack<float> {
 };
 template <> struct Pack<__nv_bfloat16> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xff80ff80u, 0xff80ff80u, 0xff80ff80u, 0xff80ff80u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         const unsigned w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
@@ -80,6 +82,7 @@ template <> struct Pack<__nv_bfloat16> {
 };
 template <> struct Pack<__half> {
     static constexpr int N = 8;
+    static __device__ __forceinline__ uint4 lowest() { return make_uint4(0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u, 0xfc00fc00u); }
     static __device__ __forceinline__ void unpack(const uint4 &r, float (&v)[N]) {
         const __half2 *p = reinterpret_cast<const __half2 *>(&r);
 #pragma unroll
@@ -251,9 +254,9 @@ __device__ __forceinline__ float2 exp_pair(float a, float b, unsigned long long 
     return make_float2(exp2_fast(e.x), exp2_fast(e.y));
 }
 
-template <typename T> __device__ __forceinline__ void add_vector(SumExp &a, const uint4 &r, float c) {
+// top: the vector's maximum; it may be NaN if an element is.
+template <typename T> __device__ __forceinline__ void add_vector(SumExp &a, const uint4 &r, float top, float c) {
     constexpr int N = Pack<T>::N;
-    const float top = Pack<T>::max(r);
     if (top > a.m) a.raise(top, c);
     float v[N];
     Pack<T>::unpack(r, v);
@@ -292,6 +295,13 @@ __device__ __forceinline__ void warp_join(SumExp &a, float c) {
     a.s = warp_sum(a.s);
 }
 
+// The part of nvec vectors that CTA `rank` of `size` has: whole 128-byte lines but for the last.
+__device__ __forceinline__ void my_part(int nvec, int rank, int size, int *v0, int *v1) {
+    const int per = (((nvec + size - 1) / size) + 7) & ~7;
+    *v0 = (int)min((long long)nvec, (long long)rank * per);
+    *v1 = (int)min((long long)nvec, (long long)(rank + 1) * per);
+}
+
 // The vectors [v0, v1) of a column, U loads in flight per thread.
 template <typename T, int THREADS, int U>
 __device__ __forceinline__ SumExp sum_exp_slice(const Column<T> &x, int v0, int v1, float c) {
@@ -303,12 +313,18 @@ __device__ __forceinline__ SumExp sum_exp_slice(const Column<T> &x, int v0, int 
 #pragma unroll
         for (int u = 0; u < U; u++) r[u] = x.load(i + u * THREADS);
 #pragma unroll
-        for (int u = 0; u < U; u++) add_vector<T>(a, r[u], c);
+        for (int u = 0; u < U; u++) add_vector<T>(a, r[u], Pack<T>::max(r[u]), c);
     }
-    for (; i < f1; i += THREADS) add_vector<T>(a, x.load(i), c);
+    for (; i < f1; i += THREADS) {
+        const uint4 r = x.load(i);
+        add_vector<T>(a, r, Pack<T>::max(r), c);
+    }
     if (threadIdx.x < 2) {
         const int p = x.partial((int)threadIdx.x, v0, v1);
-        if (p >= 0) add_vector<T>(a, x.load_partial(p), c);
+        if (p >= 0) {
+            const uint4 r = x.load_partial(p);
+            add_vector<T>(a, r, Pack<T>::max(r), c);
+        }
     }
     return a;
 }

@@ -1,19 +1,20 @@
 // The k largest logits of every token column as a sparse matrix, with the column's log-sum-exp.
 //
 // Values are compared as whole numbers in the order of the floats, and with the lower row first where they are equal.
-//
-// Columns up to 1.5 MB: a cluster of up to 8 CTAs per column, each with a part of it in shared memory.
-//   1. Each thread's vectors form one to four groups, of which it finds the largest value.  With at least k groups in a
-//      part, the k-th largest of those maxima is a bound: k values of the part are as large or larger, so nothing below
-//      the bound is among the column's k largest.  And it is tight: for values in no particular order little more than k
-//      pass it (of 16384 values in 256 groups about 70 for k = 64, 180 for k = 128).
-//   2. The values at or above the bound are collected; threads whose maximum is below it have nothing to look at.
-//      If there are too many (equal values, a part with fewer groups than k) the part's k largest are found exactly.
-//   3. The cluster's first CTA gathers what the parts have found, finds the k-th largest by bisection, and writes
-//      every entry at the place that its rank among the survivors gives.
-// So X is read once.  Bound by memory: 131072 x 2048 bf16, k = 64, with the log-sum-exp TIMEA.
-//
-// Longer columns: one CTA per column, four rounds over eight bits of the values each.
+// A CTA, or a cluster of up to 8 where columns are few, goes over a column once, 4 vectors per thread at a time (a round):
+//   1. The first round gives a bound.  Each thread's vectors form a group, or four; with at least k groups, the k-th
+//      largest of the groups' maxima is a value that k of the round's values reach, so nothing below it is among the
+//      column's k largest.  And it is tight: in no particular order, of 8192 values in 256 groups about 70 reach it for
+//      k = 64.
+//   2. A vector whose largest value is above the bound is set aside, which costs the others one comparison.  At the
+//      end of a round the vectors set aside are gone through by all threads, element by element, and what is above the
+//      bound is listed.  When the list has grown, its k-th largest entry becomes the bound.  Rows ascend from round to
+//      round, so of equal values the later ones need not be looked at once there are k.
+//   3. In the end the parts of a cluster are put together in its first CTA; what the k-th largest entry leaves (k, or a
+//      few more) goes to the place that its rank gives.
+// Bound by memory with many long columns (131072 x 2048 bf16, k = 64: TIMES), by the chain of steps with few
+// (32768 x 1 fp32, k = 40: TIME1).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
+// CTAs spent most of their time on the bounds and on waiting for the cluster.
 #include <cuda_runtime.h>
 
 #include "tokens_stream.cuh"
@@ -30,202 +31,210 @@ __device__ __forceinline__ unsigned key_of(Entry e) { return (unsigned)(e >> 32)
 __device__ __forceinline__ unsigned row_of(Entry e) { return 0xffffffffu - (unsigned)e; }
 
 struct TopArgs {
-    int nrows, k;
+    int nrows, ncols, k;
     long long ldx;
     float t, c;
     int *ir, *ic, *jc;
     float *data, *lse;
 };
 
-constexpr int kTop = 256;                   // threads of a part
-constexpr int kCollect = BIDMAT_B200_TOP_MAX_K + 64;      // entries that a part can hand on
+constexpr int kTop = 256;                                   // threads
+constexpr int kRound = 4;                                   // vectors per thread and round
+constexpr int kSlack = 64;                                  // entries beyond k that a selection may leave
+constexpr int kBatch = kTop * 8;                            // values that are listed between two looks at the length
+constexpr int kList = kBatch + BIDMAT_B200_TOP_MAX_K + kSlack;
 
-// The values of a part that pass the bound, in an order of chance.
-template <typename T>
-__device__ __forceinline__ void collect(const uint4 *kept, int n, int groups, const float (&top)[4], unsigned bound, int row0, int rows,
-                                        Entry *list, int limit, int *count) {
-    constexpr int N = Pack<T>::N;
+struct TopShared {
+    Entry list[kList];
+    uint4 aside[kTop * kRound];
+    int aside_at[kTop * kRound];
+    unsigned hist[256];
+    float2 sums[kTop / 32];
+    int length, set_aside;
+    int digit, above, inside;
+};
+
+// One of the at most two vectors of a column that are not the column's alone.
+template <typename T> __device__ __noinline__ uint4 partial_vector(const Column<T> &x, int i) { return x.load_partial(i); }
+
+// The largest b = d 2^shift that at least k of the list's n entries reach, for the first shift from 56 down in steps of
+// 8 to `last` with which no more than k + kSlack do; how many reach it.  By the whole CTA, k <= n.
+__device__ __forceinline__ Entry select(TopShared &sh, int n, int k, int last, int *reach) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    Entry b = 0;
+    int left = k;                                           // the k-th largest is the left-th of those that agree with b
+    *reach = n;
+    for (int shift = 56; shift >= last; shift -= 8) {
+        sh.hist[tid] = 0;
+        __syncthreads();
+        const Entry mask = shift == 56 ? 0 : ~(Entry)0 << (shift + 8);
+        for (int i = tid; i < n; i += kTop) {
+            const Entry e = sh.list[i];
+            if ((e & mask) == b) atomicAdd(&sh.hist[(unsigned)(e >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (tid < 32) {                                     // lane 0 has the highest eight digits
+            int own[8], sum = 0;
 #pragma unroll
-    for (int g = 0; g < 4; g++) {
-        if (g >= groups || order_key(top[g]) < bound) continue;
-        for (int i = threadIdx.x + g * kTop; i < n; i += groups * kTop) {
-            const uint4 r = kept[i];
-            if (order_key(Pack<T>::max_nan(r)) < bound) continue;
-            float v[N];
-            Pack<T>::unpack(r, v);
+            for (int i = 0; i < 8; i++) sum += own[i] = (int)sh.hist[255 - 8 * lane - i];
+            int before = sum;
 #pragma unroll
-            for (int j = 0; j < N; j++) {
-                const unsigned key = order_key(v[j]);
-                const int row = row0 + i * N + j;
-                if (key < bound || row < 0 || row >= rows) continue;
-                const int at = atomicAdd(count, 1);
-                if (at < limit) list[at] = entry_of(key, (unsigned)row);
+            for (int o = 1; o < 32; o <<= 1) {
+                const int v = __shfl_up_sync(0xffffffffu, before, o);
+                if (lane >= o) before += v;
+            }
+            before -= sum;
+            if (before < left && left <= before + sum) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    if (before < left && left <= before + own[i]) {
+                        sh.digit = 255 - 8 * lane - i;
+                        sh.above = before;
+                        sh.inside = own[i];
+                    }
+                    before += own[i];
+                }
             }
         }
+        __syncthreads();
+        b |= (Entry)sh.digit << shift;
+        left -= sh.above;
+        *reach = k - left + sh.inside;
+        if (sh.inside - left <= kSlack) break;
     }
+    return b;
 }
 
-// The part's k largest exactly (k <= values of the part): list[0 .. k).  By the whole CTA.
-template <typename T>
-__device__ __noinline__ void select_part(const uint4 *kept, int n, int row0, int rows, int k, Entry *list, unsigned *hist, int *shared) {
-    constexpr int N = Pack<T>::N;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const T *x = reinterpret_cast<const T *>(kept);
-    const int lo = row0 < 0 ? -row0 : 0, hi = min(n * N, rows - row0);          // positions that are the column's
-    unsigned prefix = 0, left = (unsigned)k;    // the k-th largest agrees with prefix; it is the left-th of those
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        hist[tid] = 0;
-        __syncthreads();
-        const unsigned mask = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int u = lo + tid; u < hi; u += kTop) {
-            const unsigned key = order_key(to_float(x[u]));
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            unsigned m = left;
-            int b = 255;
-            while (b > 0 && hist[b] < m) m -= hist[b--];
-            shared[0] = (int)(prefix | ((unsigned)b << shift));
-            shared[1] = (int)m;
-        }
-        __syncthreads();
-        prefix = (unsigned)shared[0];
-        left = (unsigned)shared[1];
-    }
+// Leaves the entries that reach b; there is room for them in front.
+__device__ __forceinline__ void keep_from(TopShared &sh, int n, Entry b) {
+    const int tid = threadIdx.x;
     __syncthreads();
-    if (tid == 0) shared[0] = 0;
+    if (tid == 0) sh.length = 0;
+    Entry mine[(kList + kTop - 1) / kTop];
+#pragma unroll
+    for (int k = 0; k < (kList + kTop - 1) / kTop; k++) mine[k] = tid + k * kTop < n ? sh.list[tid + k * kTop] : 0;
     __syncthreads();
-    unsigned equal = 0;                         // equal values in the rows before this stretch
-    for (int u0 = lo; u0 < hi; u0 += kTop) {
-        const int u = u0 + tid;
-        const unsigned key = u < hi ? order_key(to_float(x[u])) : 0u;
-        if (u < hi && key > prefix) list[atomicAdd(&shared[0], 1)] = entry_of(key, (unsigned)(row0 + u));
-        const bool tie = u < hi && key == prefix && equal < left;
-        if (__syncthreads_or(tie)) {
-            const unsigned vote = __ballot_sync(0xffffffffu, tie);
-            if (lane == 0) hist[warp] = __popc(vote);
-            __syncthreads();
-            unsigned at = equal + __popc(vote & ((1u << lane) - 1u));
-            for (int w = 0; w < warp; w++) at += hist[w];
-            if (tie && at < left) list[(unsigned)k - left + at] = entry_of(key, (unsigned)(row0 + u));
-            for (int w = 0; w < kTop / 32; w++) equal += hist[w];
-            __syncthreads();
+#pragma unroll
+    for (int k = 0; k < (kList + kTop - 1) / kTop; k++)
+        if (tid + k * kTop < n && mine[k] >= b) sh.list[atomicAdd(&sh.length, 1)] = mine[k];
+    __syncthreads();
+}
+
+// Cuts the list to its k largest and a few; what they reach.
+__device__ __noinline__ Entry cut(TopShared &sh, int k) {
+    int reach;
+    const Entry b = select(sh, sh.length, k, 0, &reach);
+    keep_from(sh, sh.length, b);
+    return b;
+}
+
+// Goes through the vectors that were set aside: what is above `bound` is listed.  Where the list gets long it is cut, and
+// what its k largest reach is the new bound; the entries of a round come in no order, so within it rows count as well.
+template <typename T> __device__ __noinline__ unsigned go_through(TopShared &sh, int row0, int rows, int k, unsigned bound) {
+    constexpr int N = Pack<T>::N, PER = kBatch / N;         // vectors per batch
+    const int n = sh.set_aside;
+    Entry from = bound == 0xffffffffu ? ~(Entry)0 : (Entry)(bound + 1) << 32;
+    for (int first = 0; first < n; first += PER) {
+        __syncthreads();
+        if (sh.length > kList - kBatch) from = max(from, cut(sh, k));
+        const int last = min(n, first + PER);
+        for (int i = first * N + (int)threadIdx.x; i < last * N; i += kTop) {
+            const unsigned key = order_key(to_float(reinterpret_cast<const T *>(sh.aside)[i]));
+            const int row = row0 + sh.aside_at[i / N] * N + (i & (N - 1));
+            const Entry e = entry_of(key, (unsigned)row);
+            if (e >= from && row >= 0 && row < rows) sh.list[atomicAdd(&sh.length, 1)] = e;
         }
     }
     __syncthreads();
+    if (threadIdx.x == 0) sh.set_aside = 0;
+    if (sh.length >= 2 * k + 256) from = max(from, cut(sh, k));
+    // later rows are larger: what equals the k-th of the list comes behind it
+    return from == (Entry)(bound + 1) << 32 ? bound : key_of(from);
 }
 
 template <typename T, bool LSE>
-__global__ void __launch_bounds__(kTop, 5) top_part_kernel(TopArgs a, Layout l, int groups, int limit, const T *X) {
-    constexpr int N = Pack<T>::N, W = kTop / 32;
-    __shared__ Entry list[kCollect];
-    __shared__ unsigned hist[kTop];
-    unsigned *maxima = reinterpret_cast<unsigned *>(list);      // of the groups, before there are entries
-    static_assert(sizeof(list) >= 4 * kTop * sizeof(unsigned), "the groups' maxima share the list's memory");
-    __shared__ float2 sums[W];
-    __shared__ int count, shared[2];
-    __shared__ unsigned bound;
-    extern __shared__ uint4 kept[];
+__global__ void __launch_bounds__(kTop, 5) top_kernel(TopArgs a, int groups, const T *X) {
+    __shared__ TopShared sh;
     cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31;
-    const int col = (int)(blockIdx.x / (unsigned)l.parts), part = (int)(blockIdx.x % (unsigned)l.parts);
-    const Slice<T> x(X, a.ldx, a.nrows, l, col, part);
-    const T *const end = X + (l.ncols - 1) * a.ldx + a.nrows;
-    x.template copy<kTop>(kept, X, end);
-    if (tid == 0) count = 0;
-    const int row0 = x.v0 * N - x.shift;                        // row of position 0
-    x.template arrive<kTop>(kept, X, end, X + col * a.ldx, a.nrows);
-
-    // 1. groups and their maxima
-    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-    if (groups == 1) {
-#pragma unroll 4
-        for (int i = tid; i < x.n; i += kTop) top[0] = larger_nan(top[0], Pack<T>::max_nan(kept[i]));
-    } else {
+    const int tid = threadIdx.x, lane = tid & 31, part = (int)cluster.block_rank(), parts = (int)cluster.num_blocks();
+    const int col = (int)(blockIdx.x / (unsigned)parts);
+    const Column<T> x(X + col * a.ldx, a.nrows);
+    int v0, v1;
+    my_part(x.nvec, part, parts, &v0, &v1);
+    const int row0 = -x.shift;                                  // row of position 0
+    if (tid == 0) sh.length = sh.set_aside = 0;
+    unsigned bound = 0;                                         // values with a larger key are wanted
+    SumExp s;
+    for (int r0 = v0; r0 < v1; r0 += kTop * kRound) {
+        uint4 r[kRound];
+        float top[kRound];
 #pragma unroll
-        for (int g = 0; g < 4; g++)
-            for (int i = tid + g * kTop; i < x.n && g < groups; i += groups * kTop) top[g] = larger_nan(top[g], Pack<T>::max_nan(kept[i]));
+        for (int k = 0; k < kRound; k++) {
+            const int i = r0 + tid + k * kTop;
+            r[k] = i >= x.full0 && i < min(x.full1, v1) ? x.load(i) : (i < v1 ? partial_vector(x, i) : Pack<T>::lowest());
+        }
+#pragma unroll
+        for (int k = 0; k < kRound; k++) {
+            top[k] = Pack<T>::max_nan(r[k]);
+            if (LSE) add_vector<T>(s, r[k], top[k], a.c);
+        }
+        unsigned first = 0;
+        if (r0 == v0) {
+            // 16 bits of the k-th largest maximum are enough; what equals them is wanted in this round
+            if (groups == kTop) {
+                sh.list[tid] = (Entry)order_key(larger_nan(larger_nan(top[0], top[1]), larger_nan(top[2], top[3]))) << 32;
+            } else {
+#pragma unroll
+                for (int k = 0; k < kRound; k++) sh.list[tid + k * kTop] = (Entry)order_key(top[k]) << 32;
+            }
+            __syncthreads();
+            int reach;
+            first = key_of(select(sh, groups, a.k, 48, &reach));
+            // groups of nothing but -infinity, or of nothing at all, give no bound
+            bound = first > order_key(-INFINITY) ? first - 1 : 0;
+        }
+        // as a float, of which NaN wants everything; 0x7fffffff, the key below zero's, would be the other zero
+        const float limit = order_value(bound == 0x7fffffffu ? bound - 1 : bound);
+#pragma unroll
+        for (int k = 0; k < kRound; k++)
+            if (!(top[k] <= limit) && r0 + tid + k * kTop < v1) {
+                const int at = atomicAdd(&sh.set_aside, 1);
+                sh.aside[at] = r[k];
+                sh.aside_at[at] = r0 + tid + k * kTop;
+            }
+        __syncthreads();
+        if (sh.set_aside > 0) {
+            const unsigned before = bound;
+            bound = go_through<T>(sh, row0, a.nrows, a.k, bound);
+            if (r0 == v0 && before > 0) bound = max(bound, first);
+        }
+        __syncthreads();
     }
-#pragma unroll
-    for (int g = 0; g < 4; g++)
-        if (g < groups) maxima[g * kTop + tid] = order_key(top[g]);
     if (LSE) {
-        SumExp s;
-        s.m = top[0];
-#pragma unroll
-        for (int g = 1; g < 4; g++) s.m = larger_nan(s.m, top[g]);
-        const float ref = s.ref();
-        const unsigned long long mr = pair(-ref, -ref), cc = pair(a.c, a.c);
-        unsigned long long acc = pair(0.f, 0.f);
-#pragma unroll 2
-        for (int i = tid; i < x.n; i += kTop) {
-            float v[N];
-            Pack<T>::unpack(kept[i], v);
-#pragma unroll
-            for (int j = 0; j < N; j += 2) {
-                const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
-                acc = add2(acc, pair(q.x, q.y));
-            }
-        }
-        const float2 q = unpair(acc);
-        s.s = q.x + q.y;
         warp_join(s, a.c);
-        if (lane == 0) sums[tid >> 5] = make_float2(s.m, s.s);
+        if (lane == 0) sh.sums[tid >> 5] = make_float2(s.m, s.s);
     }
     __syncthreads();
-    // the bound: 16 bits of the k-th largest maximum are enough
-    if (tid < 32) {
-        unsigned key[4 * kTop / 32];
-#pragma unroll
-        for (int i = 0; i < 4 * kTop / 32; i++) key[i] = i < groups * (kTop / 32) ? maxima[i * 32 + lane] : 0u;
-        unsigned b = 0;
-        for (int bit = 31; bit >= 16; bit--) {
-            const unsigned tryb = b | (1u << bit);
-            int n = 0;
-#pragma unroll
-            for (int i = 0; i < kTop / 32; i++) n += key[i] >= tryb;
-            if (groups > 1) {
-#pragma unroll
-                for (int i = kTop / 32; i < 4 * kTop / 32; i++) n += key[i] >= tryb;
-            }
-            if (__reduce_add_sync(0xffffffffu, n) >= a.k) b = tryb;
-        }
-        if (lane == 0) bound = b;
-    }
-    __syncthreads();
-    // 2. what passes it
-    collect<T>(kept, x.n, groups, top, bound, row0, a.nrows, list, limit, &count);
-    __syncthreads();
-    int found = count;
-    if (found > limit) {                                        // more than limit >= k values
-        select_part<T>(kept, x.n, row0, a.nrows, a.k, list, hist, shared);
-        found = a.k;
-    }
-    __syncthreads();
-    if (tid == 0) count = found;
-
-    // 3. the cluster's first CTA puts them together
-    if (l.parts > 1) {
+    if (sh.length > a.k + kSlack) cut(sh, a.k);
+    if (parts > 1) {
         cluster.sync();
-        if (part != 0) {
-            cluster.sync();                                     // stays until it has been read
-            return;
+        if (part == 0) {
+            for (int p = 1; p < parts; p++) {
+                const int m = *cluster.map_shared_rank(&sh.length, p);
+                if (sh.length + m > kList) cut(sh, a.k);
+                const int n = sh.length;
+                const Entry *from = cluster.map_shared_rank(sh.list, p);
+                for (int i = tid; i < m; i += kTop) sh.list[n + i] = from[i];
+                __syncthreads();
+                if (tid == 0) sh.length = n + m;
+                __syncthreads();
+            }
         }
     }
-    __syncthreads();
-    Entry *all = reinterpret_cast<Entry *>(kept);               // the part is no longer needed
-    int total = 0;
-    for (int p = 0; p < l.parts; p++) {
-        const Entry *from = p ? cluster.map_shared_rank(list, p) : list;
-        const int m = p ? *cluster.map_shared_rank(&count, p) : count;
-        for (int i = tid; i < m; i += kTop) all[total + i] = from[i];
-        total += m;
-    }
-    if (LSE && tid < 32) {
-        SumExp s;
-        for (int i = lane; i < l.parts * W; i += 32) {
-            const float2 v = *cluster.map_shared_rank(&sums[i % W], i / W);
+    if (LSE && part == 0 && tid < 32) {
+        s = SumExp();
+        for (int i = lane; i < parts * (kTop / 32); i += 32) {
+            const float2 v = *cluster.map_shared_rank(&sh.sums[i % (kTop / 32)], i / (kTop / 32));
             join(s, v.x, v.y, a.c);
         }
         warp_join(s, a.c);
@@ -234,37 +243,15 @@ __global__ void __launch_bounds__(kTop, 5) top_part_kernel(TopArgs a, Layout l, 
             a.lse[col] = (float)L;
         }
     }
-    if (l.parts > 1) cluster.sync();
-    else __syncthreads();
-    // the largest b that at least k entries reach: by value, and among equal values by row where they are many
-    if (tid < 64) hist[tid] = 0;
-    __syncthreads();
-    Entry b = 0;
-    int reach = total;
-    for (int bit = 63; bit >= 0 && (bit >= 32 ? reach > a.k : reach > a.k + 64); bit--) {
-        const Entry tryb = b | ((Entry)1 << bit);
-        int n = 0;
-        for (int i = tid; i < total; i += kTop) n += all[i] >= tryb;
-        n = __reduce_add_sync(0xffffffffu, n);
-        if (lane == 0 && n) atomicAdd(&hist[bit], (unsigned)n);
-        __syncthreads();
-        n = (int)hist[bit];
-        if (n >= a.k) {
-            b = tryb;
-            reach = n;
-        }
-    }
-    // survivors side by side, then each to its rank
-    if (tid == 0) count = 0;
-    __syncthreads();
-    for (int i = tid; i < total; i += kTop)
-        if (all[i] >= b) list[atomicAdd(&count, 1)] = all[i];
-    __syncthreads();
-    for (int i = tid; i < reach; i += kTop) {
-        const Entry e = list[i];
+    if (parts > 1) cluster.sync();                              // a part stays until it has been read
+    if (part != 0) return;
+    if (sh.length > a.k + kSlack) cut(sh, a.k);
+    const int n = sh.length;
+    for (int i = tid; i < n; i += kTop) {
+        const Entry e = sh.list[i];
         int rank = 0;
 #pragma unroll 4
-        for (int j = 0; j < reach; j++) rank += list[j] > e;
+        for (int j = 0; j < n; j++) rank += sh.list[j] > e;
         if (rank >= a.k) continue;
         const long long o = (long long)col * a.k + rank;
         a.ir[o] = (int)row_of(e);
@@ -273,142 +260,22 @@ __global__ void __launch_bounds__(kTop, 5) top_part_kernel(TopArgs a, Layout l, 
     }
     if (tid == 0) {
         a.jc[col] = col * a.k;
-        if (col == l.ncols - 1) a.jc[l.ncols] = (col + 1) * a.k;
+        if (col == a.ncols - 1) a.jc[a.ncols] = (col + 1) * a.k;
     }
 }
 
-// ---------------------------------------------------------------- longer columns
-
-constexpr int kTopThreads = 512;
-
-template <typename T>
-__global__ void __launch_bounds__(kTopThreads)
-top_long_kernel(int nrows, int ncols, const T *__restrict__ X, long long ldx, int k, float temperature,
-                  int *__restrict__ Sir, int *__restrict__ Sic, int *__restrict__ Sjc, float *__restrict__ Sdata,
-                  float *__restrict__ lse) {
-    __shared__ unsigned hist[256];
-    __shared__ unsigned long long list[BIDMAT_B200_TOP_MAX_K];
-    __shared__ double red[kTopThreads / 32];
-    __shared__ unsigned warp_cnt[kTopThreads / 32];
-    __shared__ unsigned s_prefix, s_left, s_fill;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const long long c = blockIdx.x;
-    const T *x = X + c * ldx;
-
-    unsigned prefix = 0, left = k;      // the k-th largest agrees with prefix; it is the left-th of those
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < 256; i += kTopThreads) hist[i] = 0;
-        __syncthreads();
-        const unsigned mask = shift == 24 ? 0u : ~0u << (shift + 8);
-        for (int v = tid; v < nrows; v += kTopThreads) {
-            const unsigned key = order_key(to_float(x[v]));
-            if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
-        }
-        __syncthreads();
-        if (tid == 0) {
-            unsigned n = left;
-            int b = 255;
-            while (b > 0 && hist[b] < n) n -= hist[b--];
-            s_prefix = prefix | ((unsigned)b << shift);
-            s_left = n;
-        }
-        __syncthreads();
-        prefix = s_prefix;
-        left = s_left;
-    }
-    for (int i = tid; i < BIDMAT_B200_TOP_MAX_K; i += kTopThreads) list[i] = 0;
-    if (tid == 0) s_fill = 0;
-    __syncthreads();
-    unsigned equal = 0;                 // equal values in the rows before this stretch
-    for (int v0 = 0; v0 < nrows; v0 += kTopThreads) {
-        const int v = v0 + tid;
-        const unsigned key = v < nrows ? order_key(to_float(x[v])) : 0u;
-        const unsigned long long entry = ((unsigned long long)key << 32) | (0xffffffffu - (unsigned)v);
-        if (v < nrows && key > prefix) list[atomicAdd(&s_fill, 1u)] = entry;
-        const bool tie = v < nrows && key == prefix;
-        if (__syncthreads_or(tie && equal < left)) {
-            const unsigned vote = __ballot_sync(0xffffffffu, tie);
-            if (lane == 0) warp_cnt[warp] = __popc(vote);
-            __syncthreads();
-            unsigned at = equal + __popc(vote & ((1u << lane) - 1u));
-            for (int w = 0; w < warp; w++) at += warp_cnt[w];
-            if (tie && at < left) list[k - left + at] = entry;
-            for (int w = 0; w < kTopThreads / 32; w++) equal += warp_cnt[w];
-            __syncthreads();
-        }
-    }
-    __syncthreads();
-    int n = 1;
-    while (n < k) n <<= 1;
-    for (int size = 2; size <= n; size <<= 1)
-        for (int step = size >> 1; step; step >>= 1) {
-            for (int i = tid; i < n; i += kTopThreads) {
-                const int j = i ^ step;
-                if (j > i) {
-                    const bool down = (i & size) == 0;
-                    const unsigned long long p = list[i], q = list[j];
-                    if ((p < q) == down) { list[i] = q; list[j] = p; }
-                }
-            }
-            __syncthreads();
-        }
-    for (int i = tid; i < k; i += kTopThreads) {
-        const long long o = c * k + i;
-        Sir[o] = (int)(0xffffffffu - (unsigned)list[i]);
-        Sic[o] = (int)c;
-        Sdata[o] = order_value((unsigned)(list[i] >> 32));
-    }
-    if (tid == 0) {
-        Sjc[c] = (int)(c * k);
-        if (c == ncols - 1) Sjc[ncols] = (int)((c + 1) * k);
-    }
-    if (lse) {
-        const float m = order_value((unsigned)(list[0] >> 32));
-        const float u = m == -INFINITY ? 0.f : m;
-        double s = 0.0;
-        for (int v = tid; v < nrows; v += kTopThreads) s += expf((to_float(x[v]) - u) / temperature);
-        s = warp_sum(s);
-        if (lane == 0) red[warp] = s;
-        __syncthreads();
-        if (tid == 0) {
-            for (int w = 1; w < kTopThreads / 32; w++) s += red[w];
-            lse[c] = (float)((double)u / temperature + log(s));
-        }
-    }
-}
-
-// ---------------------------------------------------------------- host side
-
-constexpr long long kPartBytes = 32768, kMostPartBytes = 196608;
-
-// Parts as in the distillation: 32 KB each where that takes 8 of them or fewer, more where columns are few.  Groups: so
-// many that the k-th largest maximum is well inside them.
-template <typename T>
-cudaError_t launch_top(const TopArgs &a, int ncols, const void *X, cudaStream_t st) {
-    const long long nvec = most_vectors<T>(X, a.ldx, a.nrows, ncols), bytes = nvec * 16;
-    long long parts = (bytes + kPartBytes - 1) / kPartBytes;
-    const long long fill = (296 + ncols - 1) / ncols, worth = (nvec + kTop - 1) / kTop;
-    if (parts < fill) parts = fill < worth ? fill : worth;
+// A CTA per column, or as many as give the machine work.
+template <typename T> cudaError_t launch_top(const TopArgs &a, const void *X, cudaStream_t st) {
+    const long long bytes = (long long)a.nrows * (long long)sizeof(T);
+    const long long fill = (592 + a.ncols - 1) / a.ncols, worth = (bytes + 8191) / 8192;
+    long long parts = fill < worth ? fill : worth;
     if (parts > 8) parts = 8;
-    const long long per = ((nvec + parts - 1) / parts + 7) & ~7LL;
-    if (per * 16 > kMostPartBytes || (long long)ncols * parts > 0x7fffffffLL) {
-        top_long_kernel<T><<<ncols, kTopThreads, 0, st>>>(a.nrows, ncols, (const T *)X, a.ldx, a.k, a.t, a.ir, a.ic, a.jc, a.data, a.lse);
-        return cudaGetLastError();
-    }
-    // what the parts hand on has to fit the place of the first one's part
-    long long limit = per * 2 / parts;
-    if (limit < a.k) limit = a.k;
-    if (limit > kCollect) limit = kCollect;
-    const size_t smem = (size_t)(per * 16 > parts * limit * 8 ? per * 16 : parts * limit * 8);
-    const int groups = a.k <= kTop / 2 ? 1 : (a.k <= kTop ? 2 : 4);
-    const auto kernel = a.lse ? top_part_kernel<T, true> : top_part_kernel<T, false>;
-    if (smem > 40000) {
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (err != cudaSuccess) return err;
-    }
+    if ((long long)a.ncols * parts > 0x7fffffffLL) parts = 1;
+    const int groups = a.k <= kTop / 2 ? kTop : kTop * kRound;
+    const auto kernel = a.lse ? top_kernel<T, true> : top_kernel<T, false>;
     cudaLaunchAttribute attr;
-    const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)(ncols * parts), kTop, (int)parts, smem, st);
-    return cudaLaunchKernelEx(&cfg, kernel, a, layout<T>(X, a.ldx, ncols, (int)parts, per), groups, (int)limit, (const T *)X);
+    const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)(a.ncols * parts), kTop, (int)parts, 0, st);
+    return cudaLaunchKernelEx(&cfg, kernel, a, groups, (const T *)X);
 }
 
 }  // namespace
@@ -423,9 +290,9 @@ extern "C" int bidmat_b200_top_logits(int nrows, int ncols, const void *X, long 
     cudaStream_t st = as_stream(stream);
     if (ncols == 0) return (int)cudaMemsetAsync(Sjc, 0, sizeof(int), st);
     if (!dense_ok(X, ldx, nrows, dtype) || !Sir || !Sic || !Sdata) return (int)cudaErrorInvalidValue;
-    const TopArgs a{nrows, k, ldx, temperature, (float)(kLog2e / (double)temperature), Sir, Sic, Sjc, Sdata, lse};
+    const TopArgs a{nrows, ncols, k, ldx, temperature, (float)(kLog2e / (double)temperature), Sir, Sic, Sjc, Sdata, lse};
     cudaError_t err = cudaSuccess;
-#define CALL_TOP(T) err = launch_top<T>(a, ncols, X, st)
+#define CALL_TOP(T) err = launch_top<T>(a, X, st)
     DISPATCH_DTYPE(dtype, CALL_TOP);
 #undef CALL_TOP
     g_launches += 1;
