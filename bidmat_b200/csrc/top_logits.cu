@@ -12,8 +12,8 @@
 //      round, so of equal values the later ones need not be looked at once there are k.
 //   3. In the end the parts of a cluster are put together in its first CTA; what the k-th largest entry leaves (k, or a
 //      few more) goes to the place that its rank gives.
-// Bound by memory with many long columns (131072 x 2048 bf16, k = 64: TIMES), by the chain of steps with few
-// (32768 x 1 fp32, k = 40: TIME1).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
+// Bound by memory with many long columns (131072 x 2048 bf16, k = 64: 176 us with the log-sum-exp, 124 us without, 82 us to read), by the chain of steps with few
+// (32768 x 1 fp32, k = 40: 9.3 us).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
 // CTAs spent most of their time on the bounds and on waiting for the cluster.
 #include <cuda_runtime.h>
 
@@ -41,13 +41,14 @@ struct TopArgs {
 constexpr int kTop = 256;                                   // threads
 constexpr int kRound = 4;                                   // vectors per thread and round
 constexpr int kSlack = 64;                                  // entries beyond k that a selection may leave
+constexpr int kDrain = 128;                                 // vectors set aside that are worth going through
 constexpr int kBatch = kTop * 8;                            // values that are listed between two looks at the length
 constexpr int kList = kBatch + BIDMAT_B200_TOP_MAX_K + kSlack;
 
 struct TopShared {
     Entry list[kList];
-    uint4 aside[kTop * kRound];
-    int aside_at[kTop * kRound];
+    uint4 aside[kTop * kRound + kDrain];
+    int aside_at[kTop * kRound + kDrain];
     unsigned hist[256];
     float2 sums[kTop / 32];
     int length, set_aside;
@@ -153,7 +154,8 @@ template <typename T> __device__ __noinline__ unsigned go_through(TopShared &sh,
 }
 
 template <typename T, bool LSE>
-__global__ void __launch_bounds__(kTop, 5) top_kernel(TopArgs a, int groups, const T *X) {
+__global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int groups, const T *X) {
+    constexpr int N = Pack<T>::N;
     __shared__ TopShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, part = (int)cluster.block_rank(), parts = (int)cluster.num_blocks();
@@ -164,15 +166,32 @@ __global__ void __launch_bounds__(kTop, 5) top_kernel(TopArgs a, int groups, con
     const int row0 = -x.shift;                                  // row of position 0
     if (tid == 0) sh.length = sh.set_aside = 0;
     unsigned bound = 0;                                         // values with a larger key are wanted
+    // as a float, of which NaN wants everything; 0x7fffffff, the key below zero's, would be the other zero
+    auto limit_of = [](unsigned key) { return order_value(key == 0x7fffffffu ? key - 1 : key); };
+    float limit = limit_of(bound);
     SumExp s;
-    for (int r0 = v0; r0 < v1; r0 += kTop * kRound) {
+    const int step = kTop * kRound, f0 = max(v0, x.full0), f1 = min(v1, x.full1);
+    auto fetch = [&](uint4 (&r)[kRound], int r0) {
+        if (r0 >= f0 && r0 + step <= f1) {
+            const T *p = x.base + (long long)(r0 + tid) * N;
+#pragma unroll
+            for (int k = 0; k < kRound; k++) r[k] = load16(p + k * kTop * N);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kRound; k++) {
+                const int i = r0 + tid + k * kTop;
+                r[k] = i >= f0 && i < f1 ? x.load(i) : (i < v1 ? partial_vector(x, i) : Pack<T>::lowest());
+            }
+        }
+    };
+    uint4 next[kRound];
+    if (v0 < v1) fetch(next, v0);
+    for (int r0 = v0; r0 < v1; r0 += step) {
         uint4 r[kRound];
         float top[kRound];
 #pragma unroll
-        for (int k = 0; k < kRound; k++) {
-            const int i = r0 + tid + k * kTop;
-            r[k] = i >= x.full0 && i < min(x.full1, v1) ? x.load(i) : (i < v1 ? partial_vector(x, i) : Pack<T>::lowest());
-        }
+        for (int k = 0; k < kRound; k++) r[k] = next[k];
+        if (r0 + step < v1) fetch(next, r0 + step);
 #pragma unroll
         for (int k = 0; k < kRound; k++) {
             top[k] = Pack<T>::max_nan(r[k]);
@@ -192,23 +211,24 @@ __global__ void __launch_bounds__(kTop, 5) top_kernel(TopArgs a, int groups, con
             first = key_of(select(sh, groups, a.k, 48, &reach));
             // groups of nothing but -infinity, or of nothing at all, give no bound
             bound = first > order_key(-INFINITY) ? first - 1 : 0;
+            limit = limit_of(bound);
         }
-        // as a float, of which NaN wants everything; 0x7fffffff, the key below zero's, would be the other zero
-        const float limit = order_value(bound == 0x7fffffffu ? bound - 1 : bound);
+        int at = 0;
 #pragma unroll
         for (int k = 0; k < kRound; k++)
-            if (!(top[k] <= limit) && r0 + tid + k * kTop < v1) {
-                const int at = atomicAdd(&sh.set_aside, 1);
+            if (!(top[k] <= limit) && (r0 + step <= v1 || r0 + tid + k * kTop < v1)) {
+                at = atomicAdd(&sh.set_aside, 1);
                 sh.aside[at] = r[k];
                 sh.aside_at[at] = r0 + tid + k * kTop;
             }
-        __syncthreads();
-        if (sh.set_aside > 0) {
+        // one barrier per round; the bound changes with what is gone through only
+        if (__syncthreads_or(at + 1 >= kDrain || r0 == v0 || r0 + step >= v1)) {
             const unsigned before = bound;
             bound = go_through<T>(sh, row0, a.nrows, a.k, bound);
             if (r0 == v0 && before > 0) bound = max(bound, first);
+            limit = limit_of(bound);
+            __syncthreads();
         }
-        __syncthreads();
     }
     if (LSE) {
         warp_join(s, a.c);
