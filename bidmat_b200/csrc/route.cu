@@ -8,18 +8,22 @@
 // sums with a bias are compared in 64 bits.
 #include <cuda_runtime.h>
 
-#include "tokens_common.cuh"
+#include "tokens_stream.cuh"
 
 using namespace bidmat;
 
 namespace {
 
-constexpr int kRouteWarps = 4;      // columns in flight per CTA, one warp each
+constexpr int kRouteWarps = 4;      // warps per CTA
+constexpr int kListed = 4;          // rows per lane that a list has room for
 
 struct RouteArgs {
     int nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm;
     long long ldx;
     float scale;
+    int stride, lists_at, doubles_at, warp_bytes;       // shared memory per warp: floats per column, bytes
+    int *ir, *ic, *jc;
+    float *data;
 };
 
 // Best (key, row) over the warp: larger key, then lower row.  row < 0: no candidate.
@@ -32,74 +36,118 @@ __device__ __forceinline__ void warp_best(double &key, int &row) {
     }
 }
 
+// The same for a column of which only the rows with an fp32 key of `cut` or more come into question: one row per lane.
+// False if there are more than 32 of them, or fewer than k.
 template <typename T>
-__global__ void __launch_bounds__(kRouteWarps * 32)
-route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bias, int *__restrict__ Sir,
-             int *__restrict__ Sic, int *__restrict__ Sjc, float *__restrict__ Sdata) {
-    extern __shared__ double route_smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long c = (long long)blockIdx.x * kRouteWarps + warp;
-    if (c >= a.ncols) return;
-    double *rank = route_smem + (size_t)warp * (a.nrows + a.ngroups);      // s + bias, -inf where unavailable
-    double *gval = rank + a.nrows;
-    const T *x = X + c * a.ldx;
-    const double inf = INFINITY;
-
-    bool bad = false;
-    double m = -inf;
-    for (int e = lane; e < a.nrows; e += 32) {
-        const double v = to_float(x[e]);
-        bad |= !(v < inf);
-        m = v > m ? v : m;
+__device__ __noinline__ bool route_few(const RouteArgs &a, const T *__restrict__ x, const float *__restrict__ bias, long long c, float cut,
+                                       const float *val, int *rows) {
+    const int lane = threadIdx.x & 31;
+    int n = 0;
+    for (int e0 = 0; e0 < a.nrows; e0 += 32) {
+        const bool in = e0 + lane < a.nrows && val[e0 + lane] >= cut;
+        const unsigned vote = __ballot_sync(0xffffffffu, in);
+        const int at = n + __popc(vote & ((1u << lane) - 1u));
+        if (in && at < 32) rows[at] = e0 + lane;
+        n += __popc(vote);
     }
-    bad = __any_sync(0xffffffffu, bad);
-    m = warp_max(m);
-    if (m == -inf) m = 0.0;
-    double sum = 0.0;
-    if (a.score == BIDMAT_B200_SOFTMAX && !bad) {
+    if (n > 32 || n < a.k) return false;
+    double m = 0.0, sum = 1.0;
+    if (a.score == BIDMAT_B200_SOFTMAX) {
+        float top = -INFINITY;
+        for (int e = lane; e < a.nrows; e += 32) top = fmaxf(top, to_float(x[e]));
+        m = warp_max((double)top);
+        sum = 0.0;
         for (int e = lane; e < a.nrows; e += 32) sum += exp((double)to_float(x[e]) - m);
         sum = warp_sum(sum);
     }
+    __syncwarp();
+    const int row = lane < n ? rows[lane] : -1;
+    double s = 0.0, key = -INFINITY;
+    if (row >= 0) {
+        const double v = to_float(x[row]);
+        s = a.score == BIDMAT_B200_SOFTMAX ? exp(v - m) / sum : 1.0 / (1.0 + exp(-v));
+        key = s + bias[row];
+    }
+    int rank = 0;
+    for (int j = 0; j < n; j++) {                   // rows ascend with the lanes
+        const double other = __shfl_sync(0xffffffffu, key, j);
+        rank += other > key || (other == key && j < lane);
+    }
+    const bool pick = row >= 0 && rank < a.k;
+    if (a.renorm) {
+        const double tot = warp_sum(pick ? s : 0.0);
+        s = tot > 0.0 ? s / tot : 0.0;
+    }
+    if (pick) {
+        const long long o = c * a.k + rank;
+        a.ir[o] = row;
+        a.data[o] = (float)(s * a.scale);
+    }
+    return true;
+}
+
+// One column by one warp with everything that is compared in 64 bits.  val: nrows floats, rank: nrows + ngroups
+// doubles of shared memory.  groups: choose the groups as well; else val is -infinity where a row is out of the running.
+template <typename T>
+__device__ __noinline__ void route_exact(const RouteArgs &a, const T *__restrict__ x, const float *__restrict__ bias, long long c,
+                                         bool groups, float *val, double *rank) {
+    const int lane = threadIdx.x & 31;
+    double *gval = rank + a.nrows;                  // rank: s + bias, -inf where out of the running
+    const double inf = INFINITY;
+    double m = -inf, sum = 0.0;
+    if (groups || a.score == BIDMAT_B200_SOFTMAX) {
+        float top = -INFINITY;
+        for (int e = lane; e < a.nrows; e += 32) {
+            const float v = to_float(x[e]);
+            top = fmaxf(top, v);
+            rank[e] = v;
+            if (groups) val[e] = v;
+        }
+        m = warp_max((double)top);
+        if (m == -inf) m = 0.0;
+        if (a.score == BIDMAT_B200_SOFTMAX) {
+            for (int e = lane; e < a.nrows; e += 32) sum += exp(rank[e] - m);
+            sum = warp_sum(sum);
+        }
+    }
+    __syncwarp();
     auto score_of = [&](int e) -> double {
         const double v = to_float(x[e]);
         return a.score == BIDMAT_B200_SOFTMAX ? exp(v - m) / sum : 1.0 / (1.0 + exp(-v));
     };
-    if (!bad) {
-        for (int e = lane; e < a.nrows; e += 32) {
-            const double v = to_float(x[e]);
-            double r = v > -inf ? score_of(e) + (bias ? (double)bias[e] : 0.0) : -inf;
-            if (r != r) r = -inf;
-            rank[e] = r;
+    const bool by_score = groups || bias;           // else the scores' own order does
+    for (int e = lane; e < a.nrows; e += 32) {
+        double r = val[e];
+        if (by_score && r > -inf) r = score_of(e) + (bias ? (double)bias[e] : 0.0);
+        else if (by_score) r = -inf;
+        if (r != r) r = -inf;
+        rank[e] = r;
+    }
+    __syncwarp();
+    if (groups) {
+        const int gsize = a.nrows / a.ngroups;
+        for (int g = lane; g < a.ngroups; g += 32) {
+            double b1 = -inf, b2 = -inf;
+            for (int e = g * gsize; e < (g + 1) * gsize; e++) {
+                const double r = rank[e];
+                if (r > b1) { b2 = b1; b1 = r; } else if (r > b2) b2 = r;
+            }
+            gval[g] = (a.grouptop == 2 && b2 > -inf) ? b1 + b2 : b1;
         }
         __syncwarp();
-        const int gsize = a.nrows / a.ngroups;
-        if (a.ngroups > 1) {
-            for (int g = lane; g < a.ngroups; g += 32) {
-                double b1 = -inf, b2 = -inf;
-                for (int e = g * gsize; e < (g + 1) * gsize; e++) {
-                    const double r = rank[e];
-                    if (r > b1) { b2 = b1; b1 = r; } else if (r > b2) b2 = r;
-                }
-                gval[g] = (a.grouptop == 2 && b2 > -inf) ? b1 + b2 : b1;
-            }
-            __syncwarp();
-            // a group stays if fewer than topgroups groups come before it
-            bool drop[BIDMAT_B200_ROUTE_MAX_ROWS / 32];
-            int n = 0;
-            for (int g = lane; g < a.ngroups; g += 32, n++) {
-                int before = 0;
-                for (int h = 0; h < a.ngroups; h++)
-                    before += gval[h] > gval[g] || (gval[h] == gval[g] && h < g);
-                drop[n] = before >= a.topgroups;
-            }
-            n = 0;
-            for (int g = lane; g < a.ngroups; g += 32, n++)
-                if (drop[n])
-                    for (int e = g * gsize; e < (g + 1) * gsize; e++) rank[e] = -inf;
-            __syncwarp();
+        // a group stays if fewer than topgroups groups come before it
+        unsigned drop = 0;
+        int n = 0;
+        for (int g = lane; g < a.ngroups; g += 32, n++) {
+            int before = 0;
+            for (int h = 0; h < a.ngroups; h++)
+                before += gval[h] > gval[g] || (gval[h] == gval[g] && h < g);
+            drop |= (before >= a.topgroups ? 1u : 0u) << n;
         }
-    } else {
-        for (int e = lane; e < a.nrows; e += 32) rank[e] = -inf;
+        n = 0;
+        for (int g = lane; g < a.ngroups; g += 32, n++)
+            if ((drop >> n) & 1u)
+                for (int e = g * gsize; e < (g + 1) * gsize; e++) rank[e] = -inf;
         __syncwarp();
     }
     // k rounds: the best one that is left; then, in the order of the rows, the others with weight zero.
@@ -112,30 +160,319 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         for (int e = lane; e < a.nrows; e += 32) {
             const double r = rank[e];
             if (r != r) continue;
-            const double v = r == -inf ? -inf : (bias ? r : (double)to_float(x[e]));
+            const double v = r == -inf || bias ? r : (double)val[e];
             if (row < 0 || v > key) { key = v; row = e; }
         }
         warp_best(key, row);
         if ((row & 31) == lane) rank[row] = NAN;
         if (lane == i) {
             pick = row;
-            w = key > -inf ? score_of(row) : 0.0;
+            w = key;
         }
         __syncwarp();
     }
+    w = lane < a.k && w > -inf ? score_of(pick) : 0.0;
     if (a.renorm) {
         const double tot = warp_sum(w);
         w = tot > 0.0 ? w / tot : 0.0;
     }
     if (lane < a.k) {
         const long long o = c * a.k + lane;
-        Sir[o] = pick;
-        Sic[o] = (int)c;
-        Sdata[o] = bad ? NAN : (float)(w * a.scale);
+        a.ir[o] = pick;
+        a.data[o] = (float)(w * a.scale);
     }
-    if (lane == 0) {
-        Sjc[c] = (int)(c * a.k);
-        if (c == a.ncols - 1) Sjc[a.ncols] = (int)((c + 1) * a.k);
+}
+
+// An entry: order key above, complement of the row below.
+typedef unsigned long long Entry;
+__device__ __forceinline__ Entry entry_of(float key, int row) { return ((Entry)order_key(key) << 32) | (0xffffffffu - (unsigned)row); }
+__device__ __forceinline__ int row_of(Entry e) { return (int)(0xffffffffu - (unsigned)e); }
+__device__ __forceinline__ float key_of(Entry e) { return order_value((unsigned)(e >> 32)); }
+
+// G lanes have a column, each every G-th of its rows.  The (k+1)-th largest of the lanes' maxima is a bound that k + 1
+// rows reach; few more do, so the rows that reach it are listed and each is ranked by counting the ones before it.
+// (Sorted lists in the lanes' registers, joined by exchanges, took 36 and 47 us for the 256 x 4096 and 160 x 65537 below.)
+//
+// Where the order is that of scores plus bias, or of groups by their scores, it is found in fp32 first.  fp32 scores are
+// off by less than 2^-20 (the exponential by 2^-22 and 2^-23 times its argument, of which the score takes back as much as
+// it grows; two more roundings), and a sum by half a step; so two sums further apart than 2^-18 + 2^-22 of their size, or
+// made of the same two numbers, are in the right order.  A column with two neighbours closer than that, one in a thousand
+// or so, goes to route_exact.
+constexpr float kNear = 3.8147e-06f, kNearPart = 2.3842e-07f;
+
+__device__ __forceinline__ bool near(float a, float b) { return !(fabsf(a - b) > kNear + kNearPart * fmaxf(fabsf(a), fabsf(b))); }
+
+template <typename T, int G, bool BIAS>
+__global__ void __launch_bounds__(kRouteWarps * 32)
+route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bias) {
+    constexpr int C = 32 / G;                       // columns per warp
+    constexpr int L = kListed * G, P = kListed;     // rows that can be listed, per column and per lane
+    extern __shared__ double route_smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (G - 1), which = lane / G;
+    const unsigned mine = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (which * G);
+    const long long c = ((long long)blockIdx.x * kRouteWarps + warp) * C + which;
+    // shared memory of the warp: the keys in fp32 (scores, or scores plus bias) and the groups of each column; one column in fp64
+    char *const base = reinterpret_cast<char *>(route_smem) + (size_t)warp * a.warp_bytes;
+    float *val = reinterpret_cast<float *>(base) + which * a.stride;
+    float *gval = val + a.nrows;
+    Entry *list = reinterpret_cast<Entry *>(base + a.lists_at) + which * 2 * L, *sorted = list + L;
+    const bool on = c < a.ncols;
+    const T *x = X + (on ? c : 0) * a.ldx;
+    const bool softmax = a.score == BIDMAT_B200_SOFTMAX;
+    // scores of all rows are needed for a bias, for groups that are not ranked by their best score alone, and for softmax
+    // weights as they are
+    const bool group_scores = a.ngroups > 1 && a.grouptop == 2;
+    const bool total = softmax && (BIAS || group_scores || !a.renorm);
+
+    bool bad = false;
+    float m = -INFINITY, sum = 0.f;
+#pragma unroll 4
+    for (int e = sub; e < a.nrows; e += G) {
+        const float v = on ? to_float(x[e]) : -INFINITY;
+        bad |= !(v < INFINITY);
+        m = fmaxf(m, v);
+        val[e] = v;
+    }
+    bad = (__ballot_sync(0xffffffffu, bad) & mine) != 0;
+    if (total) {
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m == -INFINITY || bad) m = 0.f;
+#pragma unroll 4
+        for (int e = sub; e < a.nrows; e += G) sum += exp2_fast((val[e] - m) * (float)kLog2e);
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+    }
+    const float inverse = total ? 1.f / sum : 0.f;
+    // for comparisons
+    auto quick_score = [&](float v) {
+        return softmax ? exp2_fast((v - m) * (float)kLog2e) * inverse : __fdividef(1.f, 1.f + exp2_fast(-v * (float)kLog2e));
+    };
+    // for weights
+    auto score_of = [&](float v) { return softmax ? expf(v - m) / sum : 1.f / (1.f + expf(-v)); };
+    if (BIAS) {
+#pragma unroll 4
+        for (int e = sub; e < a.nrows; e += G) {
+            const float v = val[e];
+            const float r = quick_score(v) + bias[e];
+            val[e] = v > -INFINITY && r > -INFINITY ? r : -INFINITY;
+        }
+    }
+    __syncwarp();
+    bool again = false, groups_again = false;       // two neighbours too close
+    if (a.ngroups > 1) {
+        // a lane takes whole groups; the rows in turn, from another one in each lane
+        const int size = a.nrows / a.ngroups;
+        for (int g = sub; g < a.ngroups; g += G) {
+            float b1 = -INFINITY, b2 = -INFINITY;
+            int e = g * size + g % size;
+            for (int i = 0; i < size; i++) {
+                float v = val[e];
+                if (!BIAS && group_scores && v > -INFINITY) v = quick_score(v);
+                if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) b2 = v;
+                if (++e == (g + 1) * size) e = g * size;
+            }
+            gval[g] = a.grouptop == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+        }
+        __syncwarp();
+        float worst = INFINITY, best = -INFINITY;   // of the groups kept, of those dropped
+        unsigned drop = 0;                          // of this lane's groups
+        int n = 0;
+        for (int g = sub; g < a.ngroups; g += G, n++) {
+            const float v = gval[g];
+            int before = 0;
+            for (int h = 0; h < a.ngroups; h++) {
+                const float u = gval[h];
+                before += u > v || (u == v && h < g);
+            }
+            if (before < a.topgroups) worst = fminf(worst, v);
+            else best = fmaxf(best, v), drop |= 1u << (n & 31);
+        }
+        __syncwarp();
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) {
+            worst = fminf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
+            best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
+        }
+        groups_again = (BIAS || group_scores) && best > -INFINITY && near(worst, best);
+        n = 0;
+        for (int g = sub; g < a.ngroups; g += G, n++) {
+            if (!((drop >> (n & 31)) & 1u)) continue;
+            int e = g * size + g % size;
+            for (int i = 0; i < size; i++) {
+                val[e] = -INFINITY;
+                if (++e == (g + 1) * size) e = g * size;
+            }
+        }
+        __syncwarp();
+    }
+    // the bound
+    const int before_me = (1 << sub) - 1;
+    // ... of two maxima per lane, or of one where that is plenty: the bound stays well inside them, so that few more reach it
+    const bool two = G < 32 || a.k > 12;
+    float top0 = -INFINITY, top1 = -INFINITY;
+#pragma unroll 4
+    for (int e = sub; e < a.nrows; e += 2 * G) {
+        top0 = fmaxf(top0, val[e]);
+        if (e + G < a.nrows) top1 = fmaxf(top1, val[e + G]);
+    }
+    if (!two) top0 = fmaxf(top0, top1);
+    int place0 = two && top1 > top0, place1 = top0 >= top1;
+#pragma unroll
+    for (int o = 1; o < G; o++) {
+        const int from = (sub + o) & (G - 1);
+        const float t0 = __shfl_sync(0xffffffffu, top0, from, G);
+        place0 += from < sub ? t0 >= top0 : t0 > top0;
+        if (two) {
+            const float t1 = __shfl_sync(0xffffffffu, top1, from, G);
+            place0 += from < sub ? t1 >= top0 : t1 > top0;
+            place1 += from < sub ? (t0 >= top1) + (t1 >= top1) : (t0 > top1) + (t1 > top1);
+        }
+    }
+    const int kth = min(a.k, two ? 2 * G - 1 : G - 1);
+    const unsigned who0 = __ballot_sync(0xffffffffu, place0 == kth) & mine, who1 = __ballot_sync(0xffffffffu, two && place1 == kth) & mine;
+    const float bound0 = __shfl_sync(0xffffffffu, top0, who0 ? __ffs(who0) - 1 : 0), bound1 = __shfl_sync(0xffffffffu, top1, who1 ? __ffs(who1) - 1 : 0);
+    const float bound = who0 ? bound0 : bound1;
+    // the rows that reach it
+    unsigned mask = 0;
+    float rejected = -INFINITY;
+    {
+        int i = 0;
+#pragma unroll 4
+        for (int e = sub; e < a.nrows; e += G, i++) {
+            const float v = val[e];
+            const bool in = v >= bound && v > -INFINITY;
+            mask |= (in ? 1u : 0u) << i;
+            if (BIAS && !in) rejected = fmaxf(rejected, v);
+        }
+    }
+    int at = __popc(mask);
+    const int own = at;
+#pragma unroll
+    for (int o = 1; o < G; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, at, o, G);
+        if (sub >= o) at += v;
+    }
+    int n = __shfl_sync(0xffffffffu, at, G - 1, G);
+    at -= own;
+    if (__any_sync(0xffffffffu, n > L)) {
+        // more than the list holds: those above the bound, and of those that equal it the lowest rows
+        const bool over = n > L;
+        unsigned above = 0;
+        int i = 0;
+        for (int e = sub; e < a.nrows; e += G, i++) above |= (val[e] > bound ? 1u : 0u) << i;
+        int n1 = __popc(above);
+        const int own1 = n1;
+        for (int o = 1; o < G; o <<= 1) {
+            const int v = __shfl_up_sync(0xffffffffu, n1, o, G);
+            if (sub >= o) n1 += v;
+        }
+        const int first = n1 - own1;
+        n1 = __shfl_sync(0xffffffffu, n1, G - 1, G);
+        if (over && n1 + a.k > L) again = true;     // one lane has too many of the largest
+        int taken = n1;
+        for (int e = sub; e - sub < a.nrows; e += G) {
+            const bool tie = over && !again && e < a.nrows && val[e] == bound;
+            const unsigned vote = (__ballot_sync(0xffffffffu, tie) & mine) >> (which * G);
+            const int to = taken + __popc(vote & before_me);
+            if (tie && to < L) list[to] = entry_of(bound, e);
+            taken += __popc(vote);
+        }
+        if (over) {
+            mask = again ? 0 : above;
+            at = first;
+            n = again ? 0 : min(taken, L);
+        }
+    }
+    for (; mask; mask &= mask - 1) {
+        const int e = sub + (__ffs(mask) - 1) * G;
+        list[at++] = entry_of(val[e], e);
+    }
+    __syncwarp();
+    // ranks
+    {
+        Entry en[P];
+        int rank[P];
+#pragma unroll
+        for (int p = 0; p < P; p++) {
+            en[p] = sub + p * G < n ? list[sub + p * G] : 0;
+            rank[p] = 0;
+        }
+        if (n <= G) {
+            for (int j = 0; j < n; j++) rank[0] += list[j] > en[0];
+        } else {
+            for (int j = 0; j < n; j++) {
+                const Entry other = list[j];
+#pragma unroll
+                for (int p = 0; p < P; p++) rank[p] += other > en[p];
+            }
+        }
+#pragma unroll
+        for (int p = 0; p < P; p++)
+            if (sub + p * G < n) sorted[rank[p]] = en[p];
+    }
+    __syncwarp();
+    const bool none = n == 0 && !again;
+    if (!none && n < a.k) again = true;             // fewer than k rows: the others are found there
+    const Entry pick = sub < min(a.k, n) ? sorted[sub] : 0;
+    if (BIAS) {
+        // neighbours among the picks, and the last one with what comes next
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) rejected = fmaxf(rejected, __shfl_xor_sync(0xffffffffu, rejected, o));
+        if (pick != 0) {
+            if (sub + 1 < n) {
+                const Entry q = sorted[sub + 1];
+                if (near(key_of(pick), key_of(q))) {
+                    const int r = row_of(pick), t = row_of(q);
+                    if (to_float(x[r]) != to_float(x[t]) || bias[r] != bias[t]) again = true;
+                }
+            } else if (rejected > -INFINITY && near(key_of(pick), rejected)) {
+                again = true;
+            }
+        }
+    }
+    const unsigned redo_groups = __ballot_sync(0xffffffffu, groups_again && !bad && on);
+    const bool relative = softmax && !total;        // only the picks matter: relative to the largest of them
+    const int row = none || bad || pick == 0 ? sub : row_of(pick);
+    float w = 0.f;
+    if (pick != 0 && !bad) {
+        const float v = BIAS ? to_float(x[row]) : val[row];
+        w = relative ? expf(v - val[row_of(sorted[0])]) : score_of(v);
+    }
+    float wsum = w;
+    if (a.renorm) {
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, o);
+        if (!(wsum > 1e-30f) && !none && !bad) again = true;            // sigmoids that leave the range of fp32
+    } else if (!softmax && pick != 0 && !bad && w < 1e-30f) {
+        again = true;
+    }
+    if (on && sub < a.k) {
+        const long long o = c * a.k + sub;
+        a.ir[o] = row;
+        a.ic[o] = (int)c;
+        a.data[o] = bad ? NAN : (a.renorm ? (wsum > 0.f ? w / wsum : 0.f) : w) * a.scale;
+    }
+    if (on && sub == 0) {
+        a.jc[c] = (int)(c * a.k);
+        if (c == a.ncols - 1) a.jc[a.ncols] = (int)((c + 1) * a.k);
+    }
+    // columns that fp32 cannot order
+    const unsigned redo = __ballot_sync(0xffffffffu, again && !bad && on) | redo_groups;
+    for (int w2 = 0; w2 < C; w2++) {
+        const unsigned of = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (w2 * G);
+        if (!(redo & of)) continue;
+        const float last = __shfl_sync(0xffffffffu, pick != 0 ? key_of(pick) : -INFINITY, w2 * G + a.k - 1);
+        const long long col = ((long long)blockIdx.x * kRouteWarps + warp) * C + w2;
+        const T *xc = X + col * a.ldx;
+        float *v = reinterpret_cast<float *>(base) + w2 * a.stride;
+        double *rank = reinterpret_cast<double *>(base + a.doubles_at);
+        const bool groups = (redo_groups & of) != 0;
+        __syncwarp();
+        if (groups || !BIAS || !(last > -INFINITY) ||
+            !route_few<T>(a, xc, bias, col, last - 2.f * (kNear + kNearPart * fabsf(last)), v, reinterpret_cast<int *>(rank)))
+            route_exact<T>(a, xc, bias, col, groups, v, rank);
+        __syncwarp();
     }
 }
 
@@ -193,6 +530,31 @@ route_grad_kernel(RouteArgs a, int nnz, const T *X, const int *__restrict__ Sir,
     for (int e = lane; e < a.nrows; e += 32) dX[c * lddx + e] = from_float<T>(col[e]);
 }
 
+template <typename T, int G, bool BIAS>
+cudaError_t launch_route_as(RouteArgs a, const void *X, const float *bias, cudaStream_t st) {
+    constexpr int C = 32 / G;
+    const auto kernel = route_kernel<T, G, BIAS>;
+    a.stride = ((a.nrows + a.ngroups + 31) & ~31) + 8;              // columns 8 banks apart
+    a.lists_at = C * a.stride * (int)sizeof(float);
+    a.doubles_at = a.lists_at + C * 2 * kListed * G * (int)sizeof(Entry);
+    a.warp_bytes = (a.doubles_at + (a.nrows + a.ngroups) * (int)sizeof(double) + 15) & ~15;
+    const size_t smem = (size_t)kRouteWarps * a.warp_bytes;
+    if (smem > 40000) {
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
+        if (err != cudaSuccess) return err;
+    }
+    const long long per = (long long)kRouteWarps * C;
+    kernel<<<(unsigned)((a.ncols + per - 1) / per), kRouteWarps * 32, smem, st>>>(a, (const T *)X, bias);
+    return cudaGetLastError();
+}
+
+// Eight lanes per column where each then has no more than 32 rows and one pick, a whole warp for more.
+template <typename T> cudaError_t launch_route(const RouteArgs &a, const void *X, const float *bias, cudaStream_t st) {
+    if (a.nrows <= 256 && a.k <= 8)
+        return bias ? launch_route_as<T, 8, true>(a, X, bias, st) : launch_route_as<T, 8, false>(a, X, bias, st);
+    return bias ? launch_route_as<T, 32, true>(a, X, bias, st) : launch_route_as<T, 32, false>(a, X, bias, st);
+}
+
 bool route_sizes_ok(int nrows, int ncols, int score, float scale) {
     return nrows >= 1 && nrows <= BIDMAT_B200_ROUTE_MAX_ROWS && ncols >= 0 &&
            (score == BIDMAT_B200_SOFTMAX || score == BIDMAT_B200_SIGMOID) && isfinite(scale) && scale != 0.f;
@@ -213,14 +575,9 @@ extern "C" int bidmat_b200_route(int nrows, int ncols, const void *X, long long 
     cudaStream_t st = as_stream(stream);
     if (ncols == 0) return (int)cudaMemsetAsync(Sjc, 0, sizeof(int), st);
     if (!dense_ok(X, ldx, nrows, dtype) || !Sir || !Sic || !Sdata) return (int)cudaErrorInvalidValue;
-    const RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale};
-    const unsigned grid = (unsigned)((ncols + kRouteWarps - 1) / kRouteWarps);
-    const size_t smem = (size_t)kRouteWarps * (nrows + ngroups) * sizeof(double);
+    RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale, 0, 0, 0, 0, Sir, Sic, Sjc, Sdata};
     cudaError_t err = cudaSuccess;
-#define CALL_ROUTE(T)                                                                                           \
-    err = cudaFuncSetAttribute(route_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);       \
-    if (err == cudaSuccess)                                                                                    \
-        route_kernel<T><<<grid, kRouteWarps * 32, smem, st>>>(a, (const T *)X, bias, Sir, Sic, Sjc, Sdata)
+#define CALL_ROUTE(T) err = launch_route<T>(a, X, bias, st)
     DISPATCH_DTYPE(dtype, CALL_ROUTE);
 #undef CALL_ROUTE
     if (err != cudaSuccess) return (int)err;
