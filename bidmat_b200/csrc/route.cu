@@ -21,6 +21,7 @@ struct RouteArgs {
     int nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm;
     long long ldx;
     float scale;
+    int wide;                       // columns can be read 16 bytes at a time
     int stride, lists_at, doubles_at, warp_bytes;       // shared memory per warp: floats per column, bytes
     int *ir, *ic, *jc;
     float *data;
@@ -214,7 +215,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     // shared memory of the warp: the keys in fp32 (scores, or scores plus bias) and the groups of each column; one column in fp64
     char *const base = reinterpret_cast<char *>(route_smem) + (size_t)warp * a.warp_bytes;
     float *val = reinterpret_cast<float *>(base) + which * a.stride;
-    float *gval = val + a.nrows;
+    float *gval = val + ((a.nrows + 3) & ~3);
     Entry *list = reinterpret_cast<Entry *>(base + a.lists_at) + which * 2 * L, *sorted = list + L;
     const bool on = c < a.ncols;
     const T *x = X + (on ? c : 0) * a.ldx;
@@ -224,22 +225,52 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     const bool group_scores = a.ngroups > 1 && a.grouptop == 2;
     const bool total = softmax && (BIAS || group_scores || !a.renorm);
 
+    // A lane reads 16 bytes at a time where it can.  What each of its vectors has largest falls to one of two groups.
+    constexpr int N = Pack<T>::N;
+    const int quads = (a.nrows + 3) / 4;            // of val, which is padded with -infinity
     bool bad = false;
-    float m = -INFINITY, sum = 0.f;
+    float m = -INFINITY, sum = 0.f, top0 = -INFINITY, top1 = -INFINITY;
+    if (a.wide) {
+        for (int i = sub; i * N < a.nrows; i += 2 * G) {
+            const uint4 none = Pack<T>::lowest();
+            const bool second = (i + G) * N < a.nrows;
+            const uint4 r0 = on ? *reinterpret_cast<const uint4 *>(x + i * N) : none;
+            const uint4 r1 = on && second ? *reinterpret_cast<const uint4 *>(x + (i + G) * N) : none;
+            top0 = larger_nan(top0, Pack<T>::max_nan(r0));
+            top1 = larger_nan(top1, Pack<T>::max_nan(r1));
+            float v[N];
+            Pack<T>::unpack(r0, v);
+#pragma unroll
+            for (int j = 0; j < N; j += 4) *reinterpret_cast<float4 *>(val + i * N + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            if (second) {
+                Pack<T>::unpack(r1, v);
+#pragma unroll
+                for (int j = 0; j < N; j += 4)
+                    *reinterpret_cast<float4 *>(val + (i + G) * N + j) = make_float4(v[j], v[j + 1], v[j + 2], v[j + 3]);
+            }
+        }
+    } else {
 #pragma unroll 4
-    for (int e = sub; e < a.nrows; e += G) {
-        const float v = on ? to_float(x[e]) : -INFINITY;
-        bad |= !(v < INFINITY);
-        m = fmaxf(m, v);
-        val[e] = v;
+        for (int e = sub; e < quads * 4; e += G) {
+            const float v = on && e < a.nrows ? to_float(x[e]) : -INFINITY;
+            if ((e / G) & 1) top1 = larger_nan(top1, v);
+            else top0 = larger_nan(top0, v);
+            val[e] = v;
+        }
     }
+    m = larger_nan(top0, top1);
+    bad = !(m < INFINITY);
+    __syncwarp();
     bad = (__ballot_sync(0xffffffffu, bad) & mine) != 0;
     if (total) {
 #pragma unroll
         for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
         if (m == -INFINITY || bad) m = 0.f;
-#pragma unroll 4
-        for (int e = sub; e < a.nrows; e += G) sum += exp2_fast((val[e] - m) * (float)kLog2e);
+        for (int q = sub; q < quads; q += G) {
+            const float4 v = reinterpret_cast<const float4 *>(val)[q];
+            sum += (exp2_fast((v.x - m) * (float)kLog2e) + exp2_fast((v.y - m) * (float)kLog2e)) +
+                   (exp2_fast((v.z - m) * (float)kLog2e) + exp2_fast((v.w - m) * (float)kLog2e));
+        }
 #pragma unroll
         for (int o = G / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
@@ -261,17 +292,21 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     __syncwarp();
     bool again = false, groups_again = false;       // two neighbours too close
     if (a.ngroups > 1) {
-        // a lane takes whole groups; the rows in turn, from another one in each lane
+        // a lane takes whole groups, and begins each at another row than its neighbours: another bank
         const int size = a.nrows / a.ngroups;
         for (int g = sub; g < a.ngroups; g += G) {
             float b1 = -INFINITY, b2 = -INFINITY;
-            int e = g * size + g % size;
-            for (int i = 0; i < size; i++) {
-                float v = val[e];
+            const float *member = val + g * size;
+            auto add = [&](float v) {
                 if (!BIAS && group_scores && v > -INFINITY) v = quick_score(v);
-                if (v > b1) { b2 = b1; b1 = v; } else if (v > b2) b2 = v;
-                if (++e == (g + 1) * size) e = g * size;
-            }
+                b2 = fmaxf(b2, fminf(b1, v));
+                b1 = fmaxf(b1, v);
+            };
+            const int turn = g % size;
+#pragma unroll 4
+            for (int i = turn; i < size; i++) add(member[i]);
+#pragma unroll 4
+            for (int i = 0; i < turn; i++) add(member[i]);
             gval[g] = a.grouptop == 2 && b2 > -INFINITY ? b1 + b2 : b1;
         }
         __syncwarp();
@@ -298,11 +333,12 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         n = 0;
         for (int g = sub; g < a.ngroups; g += G, n++) {
             if (!((drop >> (n & 31)) & 1u)) continue;
-            int e = g * size + g % size;
-            for (int i = 0; i < size; i++) {
-                val[e] = -INFINITY;
-                if (++e == (g + 1) * size) e = g * size;
-            }
+            float *member = val + g * size;
+            const int turn = g % size;
+#pragma unroll 4
+            for (int i = turn; i < size; i++) member[i] = -INFINITY;
+#pragma unroll 4
+            for (int i = 0; i < turn; i++) member[i] = -INFINITY;
         }
         __syncwarp();
     }
@@ -310,11 +346,16 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     const int before_me = (1 << sub) - 1;
     // ... of two maxima per lane, or of one where that is plenty: the bound stays well inside them, so that few more reach it
     const bool two = G < 32 || a.k > 12;
-    float top0 = -INFINITY, top1 = -INFINITY;
+    if (BIAS || a.ngroups > 1) {                    // other keys than the scores, or not all of them
+        // every 2 G-th row, so that a group's rows fall to as many maxima as there are
+        top0 = top1 = -INFINITY;
+        int e = sub;
 #pragma unroll 4
-    for (int e = sub; e < a.nrows; e += 2 * G) {
-        top0 = fmaxf(top0, val[e]);
-        if (e + G < a.nrows) top1 = fmaxf(top1, val[e + G]);
+        for (; e + G < 4 * quads; e += 2 * G) {
+            top0 = fmaxf(top0, val[e]);
+            top1 = fmaxf(top1, val[e + G]);
+        }
+        if (e < 4 * quads) top0 = fmaxf(top0, val[e]);
     }
     if (!two) top0 = fmaxf(top0, top1);
     int place0 = two && top1 > top0, place1 = top0 >= top1;
@@ -334,18 +375,30 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     const float bound0 = __shfl_sync(0xffffffffu, top0, who0 ? __ffs(who0) - 1 : 0), bound1 = __shfl_sync(0xffffffffu, top1, who1 ? __ffs(who1) - 1 : 0);
     const float bound = who0 ? bound0 : bound1;
     // the rows that reach it
+    // bit 4 i + j of the mask: row 4 (sub + G i) + j
     unsigned mask = 0;
     float rejected = -INFINITY;
+    const float reach = fmaxf(bound, -3.4028235e38f);       // -infinity is never listed
     {
-        int i = 0;
-#pragma unroll 4
-        for (int e = sub; e < a.nrows; e += G, i++) {
-            const float v = val[e];
-            const bool in = v >= bound && v > -INFINITY;
-            mask |= (in ? 1u : 0u) << i;
-            if (BIAS && !in) rejected = fmaxf(rejected, v);
+        int bit = 0;
+#pragma unroll 2
+        for (int q = sub; q < quads; q += G, bit += 4) {
+            const float4 v = reinterpret_cast<const float4 *>(val)[q];
+            unsigned in = 0;
+            if (v.x >= reach) in |= 1u;
+            if (v.y >= reach) in |= 2u;
+            if (v.z >= reach) in |= 4u;
+            if (v.w >= reach) in |= 8u;
+            mask |= in << bit;
+            if (BIAS) {
+                if (!(in & 1u)) rejected = fmaxf(rejected, v.x);
+                if (!(in & 2u)) rejected = fmaxf(rejected, v.y);
+                if (!(in & 4u)) rejected = fmaxf(rejected, v.z);
+                if (!(in & 8u)) rejected = fmaxf(rejected, v.w);
+            }
         }
     }
+    auto masked_row = [&](int bit) { return 4 * (sub + G * (bit >> 2)) + (bit & 3); };
     int at = __popc(mask);
     const int own = at;
 #pragma unroll
@@ -359,8 +412,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         // more than the list holds: those above the bound, and of those that equal it the lowest rows
         const bool over = n > L;
         unsigned above = 0;
-        int i = 0;
-        for (int e = sub; e < a.nrows; e += G, i++) above |= (val[e] > bound ? 1u : 0u) << i;
+        for (int i = 0; masked_row(i) < 4 * quads; i++) above |= (val[masked_row(i)] > bound ? 1u : 0u) << i;
         int n1 = __popc(above);
         const int own1 = n1;
         for (int o = 1; o < G; o <<= 1) {
@@ -385,7 +437,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         }
     }
     for (; mask; mask &= mask - 1) {
-        const int e = sub + (__ffs(mask) - 1) * G;
+        const int e = masked_row(__ffs(mask) - 1);
         list[at++] = entry_of(val[e], e);
     }
     __syncwarp();
@@ -398,8 +450,13 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
             en[p] = sub + p * G < n ? list[sub + p * G] : 0;
             rank[p] = 0;
         }
-        if (n <= G) {
-            for (int j = 0; j < n; j++) rank[0] += list[j] > en[0];
+        if (__all_sync(0xffffffffu, n <= 2 * G)) {
+#pragma unroll 2
+            for (int j = 0; j < n; j++) {
+                const Entry other = list[j];
+                rank[0] += other > en[0];
+                rank[1] += other > en[1];
+            }
         } else {
             for (int j = 0; j < n; j++) {
                 const Entry other = list[j];
@@ -534,7 +591,8 @@ template <typename T, int G, bool BIAS>
 cudaError_t launch_route_as(RouteArgs a, const void *X, const float *bias, cudaStream_t st) {
     constexpr int C = 32 / G;
     const auto kernel = route_kernel<T, G, BIAS>;
-    a.stride = ((a.nrows + a.ngroups + 31) & ~31) + 8;              // columns 8 banks apart
+    a.stride = (((a.nrows + 3) / 4 * 4 + a.ngroups + 31) & ~31) + 8;              // columns 8 banks apart
+    a.wide = is16(X) && a.nrows % Pack<T>::N == 0 && (a.ldx % Pack<T>::N == 0 || a.ncols == 1);
     a.lists_at = C * a.stride * (int)sizeof(float);
     a.doubles_at = a.lists_at + C * 2 * kListed * G * (int)sizeof(Entry);
     a.warp_bytes = (a.doubles_at + (a.nrows + a.ngroups) * (int)sizeof(double) + 15) & ~15;
@@ -575,7 +633,7 @@ extern "C" int bidmat_b200_route(int nrows, int ncols, const void *X, long long 
     cudaStream_t st = as_stream(stream);
     if (ncols == 0) return (int)cudaMemsetAsync(Sjc, 0, sizeof(int), st);
     if (!dense_ok(X, ldx, nrows, dtype) || !Sir || !Sic || !Sdata) return (int)cudaErrorInvalidValue;
-    RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale, 0, 0, 0, 0, Sir, Sic, Sjc, Sdata};
+    RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale, 0, 0, 0, 0, 0, Sir, Sic, Sjc, Sdata};
     cudaError_t err = cudaSuccess;
 #define CALL_ROUTE(T) err = launch_route<T>(a, X, bias, st)
     DISPATCH_DTYPE(dtype, CALL_ROUTE);
