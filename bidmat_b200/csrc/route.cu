@@ -21,6 +21,7 @@ struct RouteArgs {
     int nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm;
     long long ldx;
     float scale;
+    int gsize;                      // rows of a group
     int wide;                       // columns can be read 16 bytes at a time
     int stride, lists_at, doubles_at, warp_bytes;       // shared memory per warp: floats per column, bytes
     int *ir, *ic, *jc;
@@ -117,6 +118,7 @@ __device__ __noinline__ void route_exact(const RouteArgs &a, const T *__restrict
         return a.score == BIDMAT_B200_SOFTMAX ? exp(v - m) / sum : 1.0 / (1.0 + exp(-v));
     };
     const bool by_score = groups || bias;           // else the scores' own order does
+#pragma unroll 4
     for (int e = lane; e < a.nrows; e += 32) {
         double r = val[e];
         if (by_score && r > -inf) r = score_of(e) + (bias ? (double)bias[e] : 0.0);
@@ -126,7 +128,7 @@ __device__ __noinline__ void route_exact(const RouteArgs &a, const T *__restrict
     }
     __syncwarp();
     if (groups) {
-        const int gsize = a.nrows / a.ngroups;
+        const int gsize = a.gsize;
         for (int g = lane; g < a.ngroups; g += 32) {
             double b1 = -inf, b2 = -inf;
             for (int e = g * gsize; e < (g + 1) * gsize; e++) {
@@ -151,26 +153,68 @@ __device__ __noinline__ void route_exact(const RouteArgs &a, const T *__restrict
                 for (int e = g * gsize; e < (g + 1) * gsize; e++) rank[e] = -inf;
         __syncwarp();
     }
-    // k rounds: the best one that is left; then, in the order of the rows, the others with weight zero.
-    // NaN marks a row that is taken.
-    double w = 0.0;
+    double w = -inf;
     int pick = 0;
-    for (int i = 0; i < a.k; i++) {
+    // The k-th largest of the lanes' maxima is a bound that k rows reach; if no more than 32 do, each is ranked by counting.
+    auto key_of_row = [&](int e) { return rank[e] == -inf || bias ? rank[e] : (double)val[e]; };
+    double top = -inf;
+    for (int e = lane; e < a.nrows; e += 32) top = fmax(top, key_of_row(e));
+    int place = 0;
+#pragma unroll 4
+    for (int j = 0; j < 32; j++) {
+        const double t = __shfl_sync(0xffffffffu, top, j);
+        place += t > top || (t == top && j < lane);
+    }
+    const double reach = __shfl_sync(0xffffffffu, top, __ffs(__ballot_sync(0xffffffffu, place == a.k - 1)) - 1);
+    int n = 0;
+    for (int e = lane; e < a.nrows; e += 32) n += key_of_row(e) >= reach ? 1 : 0;
+    n = __reduce_add_sync(0xffffffffu, n);
+    if (reach > -inf && n <= 32) {
         double key = -inf;
-        int row = -1;
-        for (int e = lane; e < a.nrows; e += 32) {
-            const double r = rank[e];
-            if (r != r) continue;
-            const double v = r == -inf || bias ? r : (double)val[e];
-            if (row < 0 || v > key) { key = v; row = e; }
+        int row = -1, have = 0;
+        for (int e0 = 0; e0 < a.nrows; e0 += 32) {  // lane i gets the i-th of them, in the order of the rows
+            const bool in = e0 + lane < a.nrows && key_of_row(e0 + lane) >= reach;
+            unsigned vote = __ballot_sync(0xffffffffu, in);
+            const int more = __popc(vote);
+            if (lane >= have && lane < have + more) {
+                for (int i = have; i < lane; i++) vote &= vote - 1;
+                row = e0 + __ffs(vote) - 1;
+                key = key_of_row(row);
+            }
+            have += more;
         }
-        warp_best(key, row);
-        if ((row & 31) == lane) rank[row] = NAN;
-        if (lane == i) {
-            pick = row;
-            w = key;
+        int r = 0;
+        for (int j = 0; j < n; j++) {
+            const double t = __shfl_sync(0xffffffffu, key, j);
+            r += t > key || (t == key && j < lane);
         }
-        __syncwarp();
+        for (int j = 0; j < n; j++) {               // rank i goes to lane i
+            const int at = __shfl_sync(0xffffffffu, r, j), from = __shfl_sync(0xffffffffu, row, j);
+            if (at == lane) {
+                pick = from;
+                w = 0.0;                            // a pick
+            }
+        }
+    } else {
+        // k rounds: the best one that is left; then, in the order of the rows, the others with weight zero.
+        // NaN marks a row that is taken.
+        for (int i = 0; i < a.k; i++) {
+            double key = -inf;
+            int row = -1;
+            for (int e = lane; e < a.nrows; e += 32) {
+                const double r = rank[e];
+                if (r != r) continue;
+                const double v = r == -inf || bias ? r : (double)val[e];
+                if (row < 0 || v > key) { key = v; row = e; }
+            }
+            warp_best(key, row);
+            if ((row & 31) == lane) rank[row] = NAN;
+            if (lane == i) {
+                pick = row;
+                w = key;
+            }
+            __syncwarp();
+        }
     }
     w = lane < a.k && w > -inf ? score_of(pick) : 0.0;
     if (a.renorm) {
@@ -194,14 +238,17 @@ __device__ __forceinline__ float key_of(Entry e) { return order_value((unsigned)
 // rows reach; few more do, so the rows that reach it are listed and each is ranked by counting the ones before it.
 // (Sorted lists in the lanes' registers, joined by exchanges, took 36 and 47 us for the 256 x 4096 and 160 x 65537 below.)
 //
-// Where the order is that of scores plus bias, or of groups by their scores, it is found in fp32 first.  fp32 scores are
-// off by less than 2^-20 (the exponential by 2^-22 and 2^-23 times its argument, of which the score takes back as much as
-// it grows; two more roundings), and a sum by half a step; so two sums further apart than 2^-18 + 2^-22 of their size, or
-// made of the same two numbers, are in the right order.  A column with two neighbours closer than that, one in a thousand
-// or so, goes to route_exact.
-constexpr float kNear = 3.8147e-06f, kNearPart = 2.3842e-07f;
+// Where the order is that of scores plus bias, or of groups by their scores, it is found in fp32 first.  A sigmoid
+// s = 1/(1 + e) is then off by at most s (1 - s) (2^-22 + |x| 2^-23) + 1.5 s 2^-23 < 2^-22 (the exponential, the sum and the
+// reciprocal), a softmax by at most 2^-20 of the column's largest (the sum's error besides).  Two sums of two of them that
+// differ by more than four times that, or sums with a bias that differ by more than twice that, and by more than
+// 2^-22 of their size for the roundings of the sums, are in the right order; so are keys made of the same two numbers.  A column
+// with two neighbours closer than that, one in some thousand, goes to route_few or route_exact.
+constexpr float kNearSigmoid = 9.5367432e-07f, kNearSoftmax = 3.8146973e-06f, kNearPart = 2.3841858e-07f;
 
-__device__ __forceinline__ bool near(float a, float b) { return !(fabsf(a - b) > kNear + kNearPart * fmaxf(fabsf(a), fabsf(b))); }
+__device__ __forceinline__ bool near(float a, float b, float within) {
+    return !(fabsf(a - b) > within + kNearPart * fmaxf(fabsf(a), fabsf(b)));
+}
 
 template <typename T, int G, bool BIAS>
 __global__ void __launch_bounds__(kRouteWarps * 32)
@@ -275,6 +322,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         for (int o = G / 2; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
     }
     const float inverse = total ? 1.f / sum : 0.f;
+    const float within = softmax ? kNearSoftmax * fminf(inverse, 1.f) : kNearSigmoid;
     // for comparisons
     auto quick_score = [&](float v) {
         return softmax ? exp2_fast((v - m) * (float)kLog2e) * inverse : __fdividef(1.f, 1.f + exp2_fast(-v * (float)kLog2e));
@@ -292,8 +340,9 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     __syncwarp();
     bool again = false, groups_again = false;       // two neighbours too close
     if (a.ngroups > 1) {
-        // a lane takes whole groups, and begins each at another row than its neighbours: another bank
-        const int size = a.nrows / a.ngroups;
+        // a lane takes whole groups; where their sizes would meet in one bank it begins each at another row than its neighbours
+        const int size = a.gsize;
+        auto first_of = [&](int g) { return (size & 7) ? 0 : (g < size ? g : g % size); };
         for (int g = sub; g < a.ngroups; g += G) {
             float b1 = -INFINITY, b2 = -INFINITY;
             const float *member = val + g * size;
@@ -302,7 +351,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
                 b2 = fmaxf(b2, fminf(b1, v));
                 b1 = fmaxf(b1, v);
             };
-            const int turn = g % size;
+            const int turn = first_of(g);
 #pragma unroll 4
             for (int i = turn; i < size; i++) add(member[i]);
 #pragma unroll 4
@@ -329,12 +378,12 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
             worst = fminf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
             best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
         }
-        groups_again = (BIAS || group_scores) && best > -INFINITY && near(worst, best);
+        groups_again = (BIAS || group_scores) && best > -INFINITY && near(worst, best, within);
         n = 0;
         for (int g = sub; g < a.ngroups; g += G, n++) {
             if (!((drop >> (n & 31)) & 1u)) continue;
             float *member = val + g * size;
-            const int turn = g % size;
+            const int turn = first_of(g);
 #pragma unroll 4
             for (int i = turn; i < size; i++) member[i] = -INFINITY;
 #pragma unroll 4
@@ -479,11 +528,11 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         if (pick != 0) {
             if (sub + 1 < n) {
                 const Entry q = sorted[sub + 1];
-                if (near(key_of(pick), key_of(q))) {
+                if (near(key_of(pick), key_of(q), within)) {
                     const int r = row_of(pick), t = row_of(q);
                     if (to_float(x[r]) != to_float(x[t]) || bias[r] != bias[t]) again = true;
                 }
-            } else if (rejected > -INFINITY && near(key_of(pick), rejected)) {
+            } else if (rejected > -INFINITY && near(key_of(pick), rejected, within)) {
                 again = true;
             }
         }
@@ -520,6 +569,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         const unsigned of = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (w2 * G);
         if (!(redo & of)) continue;
         const float last = __shfl_sync(0xffffffffu, pick != 0 ? key_of(pick) : -INFINITY, w2 * G + a.k - 1);
+        const float cut = last - 2.f * (__shfl_sync(0xffffffffu, within, w2 * G) + kNearPart * fabsf(last));
         const long long col = ((long long)blockIdx.x * kRouteWarps + warp) * C + w2;
         const T *xc = X + col * a.ldx;
         float *v = reinterpret_cast<float *>(base) + w2 * a.stride;
@@ -527,7 +577,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         const bool groups = (redo_groups & of) != 0;
         __syncwarp();
         if (groups || !BIAS || !(last > -INFINITY) ||
-            !route_few<T>(a, xc, bias, col, last - 2.f * (kNear + kNearPart * fabsf(last)), v, reinterpret_cast<int *>(rank)))
+            !route_few<T>(a, xc, bias, col, cut, v, reinterpret_cast<int *>(rank)))
             route_exact<T>(a, xc, bias, col, groups, v, rank);
         __syncwarp();
     }
@@ -633,7 +683,7 @@ extern "C" int bidmat_b200_route(int nrows, int ncols, const void *X, long long 
     cudaStream_t st = as_stream(stream);
     if (ncols == 0) return (int)cudaMemsetAsync(Sjc, 0, sizeof(int), st);
     if (!dense_ok(X, ldx, nrows, dtype) || !Sir || !Sic || !Sdata) return (int)cudaErrorInvalidValue;
-    RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale, 0, 0, 0, 0, 0, Sir, Sic, Sjc, Sdata};
+    RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale, nrows / ngroups, 0, 0, 0, 0, 0, Sir, Sic, Sjc, Sdata};
     cudaError_t err = cudaSuccess;
 #define CALL_ROUTE(T) err = launch_route<T>(a, X, bias, st)
     DISPATCH_DTYPE(dtype, CALL_ROUTE);
