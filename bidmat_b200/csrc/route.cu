@@ -22,7 +22,7 @@ struct RouteArgs {
     long long ldx;
     float scale;
     int gsize;                      // rows of a group
-    int wide;                       // columns can be read 16 bytes at a time
+    int wide, wide_out;             // columns can be read, written 16 bytes at a time
     int stride, lists_at, doubles_at, warp_bytes;       // shared memory per warp: floats per column, bytes
     int *ir, *ic, *jc;
     float *data;
@@ -586,55 +586,119 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
 // The gradient of the weights goes back to the scores (w, g: weight and gradient of an entry, D = sum of w g):
 //   softmax, renormalised: w (g - D/scale)            sigmoid, renormalised: w (1 - s) (g - D/scale)
 //   softmax:  w g at the entries, - p D everywhere    sigmoid:               w (1 - s) g
-template <typename T>
+//
+// G lanes have a column.  It is put together in shared memory in fp32: what every row gets, then the entries, one lane at a
+// time, so that a row that comes twice gets its terms in their order.  Bound by memory for many columns (160 x 65537 bf16,
+// softmax: 17.6 us for 7.2 us of copying), by latency for few (256 x 4096 fp32: 3.5 us).
+template <typename T, int G>
 __global__ void __launch_bounds__(kRouteWarps * 32)
-route_grad_kernel(RouteArgs a, int nnz, const T *X, const int *__restrict__ Sir,
-                  const int *__restrict__ Sjc, const float *__restrict__ Sdata, const float *__restrict__ dS,
-                  T *dX, long long lddx) {
-    extern __shared__ float route_grad_smem[];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const long long c = (long long)blockIdx.x * kRouteWarps + warp;
-    if (c >= a.ncols) return;
-    float *col = route_grad_smem + (size_t)warp * a.nrows;
-    const T *x = X + c * a.ldx;
-    const int j0 = max(Sjc[c], 0), j1 = min(Sjc[c + 1], nnz);
-    float d = 0.f;
-    for (int j = j0 + lane; j < j1; j += 32) d = fmaf(Sdata[j], dS[j], d);
-    d = warp_sum(d);
-    if (a.score == BIDMAT_B200_SOFTMAX && !a.renorm) {
-        float m = -INFINITY, sum = 0.f;
-        for (int e = lane; e < a.nrows; e += 32) m = fmaxf(m, to_float(x[e]));
+route_grad_kernel(RouteArgs a, int nnz, const T *X, const int *__restrict__ Sir, const int *__restrict__ Sjc,
+                  const float *__restrict__ Sdata, const float *__restrict__ dS, T *dX, long long lddx) {
+    constexpr int C = 32 / G, N = Pack<T>::N, V = 32 / N;       // columns per warp, vectors per lane: 32 G rows at most
+    extern __shared__ float4 route_grad_smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane & (G - 1), which = lane / G;
+    const long long c = ((long long)blockIdx.x * kRouteWarps + warp) * C + which;
+    const bool on = c < a.ncols;
+    float *col = reinterpret_cast<float *>(route_grad_smem) + (size_t)(warp * C + which) * a.stride;
+    const T *x = X + (on ? c : 0) * a.ldx;
+    const int j0 = on ? max(Sjc[c], 0) : 0, j1 = on ? min(Sjc[c + 1], nnz) : 0;
+    const bool everywhere = a.score == BIDMAT_B200_SOFTMAX && !a.renorm;
+    auto over_lanes = [&](float v) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-        if (m == -INFINITY) m = 0.f;
-        for (int e = lane; e < a.nrows; e += 32) {
-            const float v = expf(to_float(x[e]) - m);
-            col[e] = v;
-            sum += v;
+        for (int o = G / 2; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+        return v;
+    };
+    uint4 r[V];
+    if (everywhere) {
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            const int i = sub + k * G;
+            r[k] = Pack<T>::lowest();
+            if (on && i * N < a.nrows) {
+                if (a.wide) {
+                    r[k] = *reinterpret_cast<const uint4 *>(x + i * N);
+                } else {
+                    float v[N];
+#pragma unroll
+                    for (int j = 0; j < N; j++) v[j] = i * N + j < a.nrows ? to_float(x[i * N + j]) : -INFINITY;
+                    r[k] = Pack<T>::pack(v);
+                }
+            }
         }
-        sum = warp_sum(sum);
+    }
+    float d = 0.f;
+    for (int j = j0 + sub; j < j1; j += G) d = fmaf(Sdata[j], dS[j], d);
+    d = over_lanes(d);
+    if (everywhere) {
+        float m = -INFINITY, sum = 0.f;
+#pragma unroll
+        for (int k = 0; k < V; k++) m = fmaxf(m, Pack<T>::max(r[k]));
+#pragma unroll
+        for (int o = G / 2; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+        if (m == -INFINITY) m = 0.f;
+        const unsigned long long mr = pair(-m, -m), cc = pair((float)kLog2e, (float)kLog2e);
+        float e[V * N];
+#pragma unroll
+        for (int k = 0; k < V; k++) {
+            float v[N];
+            Pack<T>::unpack(r[k], v);
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
+                e[k * N + j] = q.x;
+                e[k * N + j + 1] = q.y;
+                sum += q.x + q.y;
+            }
+        }
+        sum = over_lanes(sum);
         const float f = sum > 0.f ? -d / sum : (sum == 0.f ? 0.f : NAN);
-        for (int e = lane; e < a.nrows; e += 32) col[e] *= f;
+#pragma unroll
+        for (int k = 0; k < V; k++)
+            if ((sub + k * G) * N < a.nrows)
+#pragma unroll
+                for (int j = 0; j < N; j += 4)
+                    *reinterpret_cast<float4 *>(col + (sub + k * G) * N + j) =
+                        make_float4(e[k * N + j] * f, e[k * N + j + 1] * f, e[k * N + j + 2] * f, e[k * N + j + 3] * f);
     } else {
-        for (int e = lane; e < a.nrows; e += 32) col[e] = 0.f;
+        for (int i = sub; i * 4 < a.nrows; i += G) *reinterpret_cast<float4 *>(col + i * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncwarp();
     const float back = a.renorm ? d / a.scale : 0.f;
-    for (int j = j0; j < j1; j += 32) {
-        const bool on = j + lane < j1;
-        const int row = on ? Sir[j + lane] : -1;
+    for (int j = j0; __any_sync(0xffffffffu, j < j1); j += G) {
+        const bool have = j + sub < j1;
+        const int row = have ? Sir[j + sub] : -1;
+        const bool in = row >= 0 && row < a.nrows;
         float v = 0.f;
-        if (row >= 0 && row < a.nrows) {
-            v = Sdata[j + lane] * (dS[j + lane] - back);
+        if (in) {
+            v = Sdata[j + sub] * (dS[j + sub] - back);
             if (a.score == BIDMAT_B200_SIGMOID) v *= 1.f / (1.f + expf(to_float(x[row])));
         }
-        // one lane at a time: a row that comes twice gets its terms in their order
-        for (int l = 0; l < min(32, j1 - j); l++) {
-            if (l == lane && row >= 0 && row < a.nrows) col[row] += v;
+        const int most = __reduce_max_sync(0xffffffffu, min(j1 - j, G));
+        for (int l = 0; l < most; l++) {
+            if (l == sub && in) col[row] += v;
             __syncwarp();
         }
     }
-    for (int e = lane; e < a.nrows; e += 32) dX[c * lddx + e] = from_float<T>(col[e]);
+    if (!on) return;
+    T *out = dX + c * lddx;
+    for (int i = sub; i * N < a.nrows; i += G) {
+        float v[N];
+#pragma unroll
+        for (int j = 0; j < N; j += 4) {
+            const float4 q = *reinterpret_cast<const float4 *>(col + i * N + j);
+            v[j] = q.x;
+            v[j + 1] = q.y;
+            v[j + 2] = q.z;
+            v[j + 3] = q.w;
+        }
+        if (a.wide_out) {
+            store16(out + i * N, Pack<T>::pack(v));
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; j++)
+                if (i * N + j < a.nrows) out[i * N + j] = from_float<T>(v[j]);
+        }
+    }
 }
 
 template <typename T, int G, bool BIAS>
@@ -663,6 +727,27 @@ template <typename T> cudaError_t launch_route(const RouteArgs &a, const void *X
     return bias ? launch_route_as<T, 32, true>(a, X, bias, st) : launch_route_as<T, 32, false>(a, X, bias, st);
 }
 
+template <typename T, int G>
+cudaError_t launch_grad_as(RouteArgs a, int nnz, const void *X, const int *Sir, const int *Sjc, const float *Sdata, const float *dS,
+                           void *dX, long long lddx, cudaStream_t st) {
+    constexpr int N = Pack<T>::N;
+    a.stride = ((a.nrows + 31) & ~31) + 8;
+    a.wide = is16(X) && a.nrows % N == 0 && (a.ldx % N == 0 || a.ncols == 1);
+    a.wide_out = is16(dX) && a.nrows % N == 0 && (lddx % N == 0 || a.ncols == 1);
+    const size_t smem = (size_t)kRouteWarps * (32 / G) * a.stride * sizeof(float);
+    const long long per = (long long)kRouteWarps * (32 / G);
+    route_grad_kernel<T, G><<<(unsigned)((a.ncols + per - 1) / per), kRouteWarps * 32, smem, st>>>(a, nnz, (const T *)X, Sir, Sjc, Sdata, dS,
+                                                                                                (T *)dX, lddx);
+    return cudaGetLastError();
+}
+
+template <typename T>
+cudaError_t launch_grad(const RouteArgs &a, int nnz, const void *X, const int *Sir, const int *Sjc, const float *Sdata, const float *dS,
+                        void *dX, long long lddx, cudaStream_t st) {
+    return a.nrows <= 256 ? launch_grad_as<T, 8>(a, nnz, X, Sir, Sjc, Sdata, dS, dX, lddx, st)
+                          : launch_grad_as<T, 32>(a, nnz, X, Sir, Sjc, Sdata, dS, dX, lddx, st);
+}
+
 bool route_sizes_ok(int nrows, int ncols, int score, float scale) {
     return nrows >= 1 && nrows <= BIDMAT_B200_ROUTE_MAX_ROWS && ncols >= 0 &&
            (score == BIDMAT_B200_SOFTMAX || score == BIDMAT_B200_SIGMOID) && isfinite(scale) && scale != 0.f;
@@ -683,7 +768,7 @@ extern "C" int bidmat_b200_route(int nrows, int ncols, const void *X, long long 
     cudaStream_t st = as_stream(stream);
     if (ncols == 0) return (int)cudaMemsetAsync(Sjc, 0, sizeof(int), st);
     if (!dense_ok(X, ldx, nrows, dtype) || !Sir || !Sic || !Sdata) return (int)cudaErrorInvalidValue;
-    RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale, nrows / ngroups, 0, 0, 0, 0, 0, Sir, Sic, Sjc, Sdata};
+    RouteArgs a{nrows, ncols, k, score, ngroups, topgroups, grouptop, renorm, ldx, scale, nrows / ngroups, 0, 0, 0, 0, 0, 0, Sir, Sic, Sjc, Sdata};
     cudaError_t err = cudaSuccess;
 #define CALL_ROUTE(T) err = launch_route<T>(a, X, bias, st)
     DISPATCH_DTYPE(dtype, CALL_ROUTE);
@@ -704,12 +789,10 @@ extern "C" int bidmat_b200_route_grad(int nrows, int ncols, int nnz, const void 
     cudaStream_t st = as_stream(stream);
     RouteArgs a{};
     a.nrows = nrows; a.ncols = ncols; a.score = score; a.renorm = renorm; a.ldx = ldx; a.scale = scale;
-    const unsigned grid = (unsigned)((ncols + kRouteWarps - 1) / kRouteWarps);
-    const size_t smem = (size_t)kRouteWarps * nrows * sizeof(float);
-#define CALL_GRAD(T)                                                                                               \
-    route_grad_kernel<T><<<grid, kRouteWarps * 32, smem, st>>>(a, nnz, (const T *)X, Sir, Sjc, Sdata, dS, (T *)dX, lddx)
+    cudaError_t err = cudaSuccess;
+#define CALL_GRAD(T) err = launch_grad<T>(a, nnz, X, Sir, Sjc, Sdata, dS, dX, lddx, st)
     DISPATCH_DTYPE(dtype, CALL_GRAD);
 #undef CALL_GRAD
     g_launches += 1;
-    return (int)cudaGetLastError();
+    return (int)err;
 }
