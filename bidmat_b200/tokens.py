@@ -25,6 +25,9 @@ from .mat import GHMat, GMat, GSMat, _check, _ptr
 
 _L = _lib.lib
 
+# torch.cuda.current_stream(i).cuda_stream without making the stream object, which takes as long as the rest of a call
+_raw_stream = torch._C._cuda_getCurrentRawStream
+
 F32, BF16, F16 = 0, 1, 2
 _DTYPES = {torch.float32: F32, torch.bfloat16: BF16, torch.float16: F16}
 _SCORES = {"softmax": 0, "sigmoid": 1}
@@ -79,10 +82,12 @@ def _new_sparse(X, k, omat, what):
     dev = X.t.device
     if nnz > 0x7fffffff:
         raise RuntimeError("%s: %d entries do not fit 32-bit indices" % (what, nnz))
-    return GSMat(X.nrows, X.ncols, nnz, torch.empty(nnz, dtype=torch.int32, device=dev),
-                 torch.empty(nnz, dtype=torch.int32, device=dev),
-                 torch.empty(X.ncols + 1, dtype=torch.int32, device=dev),
-                 torch.empty(nnz, dtype=torch.float32, device=dev))
+    # one allocation; the lists begin at multiples of 16 bytes
+    n4 = (nnz + 3) & ~3
+    pir, pic, data, pjc = torch.empty(3 * n4 + X.ncols + 1, dtype=torch.int32, device=dev).split((n4, n4, n4, X.ncols + 1))
+    if n4 != nnz:
+        pir, pic, data = pir[:nnz], pic[:nnz], data[:nnz]
+    return GSMat(X.nrows, X.ncols, nnz, pir, pic, pjc, data.view(torch.float32))
 
 
 def _new_dense(X, omat, what):
@@ -100,8 +105,13 @@ def _row(ncols, device):
 
 
 def _call(fn, device, what, *args):
-    with torch.cuda.device(device):
-        _check(fn(*args, torch.cuda.current_stream().cuda_stream), what)
+    if device.index == torch.cuda.current_device():
+        err = fn(*args, _raw_stream(device.index))
+    else:
+        with torch.cuda.device(device):
+            err = fn(*args, _raw_stream(device.index))
+    if err != 0:
+        _check(err, what)
 
 
 def route(X, k, score="softmax", bias=None, groups=1, topgroups=1, grouptop=2, renorm=True, scale=1.0, omat=None):
