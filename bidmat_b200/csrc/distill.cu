@@ -549,8 +549,11 @@ cudaError_t launch_distill(const DistillArgs &a, int ncols, const void *X, void 
 // enough of them (131072 x 2048 bf16: 89 us in one part, 106 us in two, 126 us in four).
 template <typename T> cudaError_t launch_loss(const DistillArgs &a, int ncols, const void *X, cudaStream_t st) {
     const long long bytes = (long long)a.nrows * (long long)sizeof(T);
-    const long long fill = (592 + ncols - 1) / ncols, worth = (bytes + 8191) / 8192, parts = fill < worth ? fill : worth;
-    return launch_long<T, false>(a, ncols, (int)(parts < 8 ? parts : 8), X, nullptr, st);
+    const long long fill = 888 / ncols, worth = (bytes + 8191) / 8192;      // six per SM
+    long long parts = fill < worth ? fill : worth;
+    if (parts < 1) parts = 1;
+    if (parts > 8) parts = 8;
+    return launch_long<T, false>(a, ncols, (int)parts, X, nullptr, st);
 }
 
 DistillArgs arguments(int nrows, long long ldx, long long lddx, float t, const Teacher &z, const float *weights, const float *lse_in,
@@ -561,7 +564,7 @@ DistillArgs arguments(int nrows, long long ldx, long long lddx, float t, const T
 int check(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype, float temperature, const int *Zir,
           const int *Zjc, const float *Zdata) {
     if (nrows < 1 || nrows > kMostRows || ncols < 0 || ncols > kMostRows || nnz < 0 || !dtype_ok(dtype)) return (int)cudaErrorInvalidValue;
-    if (!isfinite(temperature) || temperature <= 0.f) return (int)cudaErrorInvalidValue;
+    if (!temperature_ok(temperature)) return (int)cudaErrorInvalidValue;
     if (ncols == 0) return 0;
     if (!dense_ok(X, ldx, nrows, dtype) || !Zjc || (nnz > 0 && (!Zir || !Zdata))) return (int)cudaErrorInvalidValue;
     return 0;
@@ -581,7 +584,7 @@ extern "C" int bidmat_b200_distill(int nrows, int ncols, int nnz, const void *X,
 #define CALL_LOSS(T) err = launch_loss<T>(a, ncols, X, as_stream(stream))
     DISPATCH_DTYPE(dtype, CALL_LOSS);
 #undef CALL_LOSS
-    g_launches += 1;
+    if (err == cudaSuccess) g_launches += 1;
     return (int)err;
 }
 
@@ -599,7 +602,7 @@ extern "C" int bidmat_b200_distill_grad(int nrows, int ncols, int nnz, const voi
 #define CALL_GRAD(T) err = launch_distill<T, GRAD>(a, ncols, X, dX, as_stream(stream))
     DISPATCH_DTYPE(dtype, CALL_GRAD);
 #undef CALL_GRAD
-    g_launches += 1;
+    if (err == cudaSuccess) g_launches += 1;
     return (int)err;
 }
 
@@ -617,6 +620,6 @@ extern "C" int bidmat_b200_distill_with_grad(int nrows, int ncols, int nnz, cons
 #define CALL_BOTH(T) err = launch_distill<T, BOTH>(a, ncols, X, dX, as_stream(stream))
     DISPATCH_DTYPE(dtype, CALL_BOTH);
 #undef CALL_BOTH
-    g_launches += 1;
+    if (err == cudaSuccess) g_launches += 1;
     return (int)err;
 }

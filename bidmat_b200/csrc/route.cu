@@ -793,6 +793,6 @@ extern "C" int bidmat_b200_route_grad(int nrows, int ncols, int nnz, const void 
 #define CALL_GRAD(T) err = launch_grad<T>(a, nnz, X, Sir, Sjc, Sdata, dS, dX, lddx, st)
     DISPATCH_DTYPE(dtype, CALL_GRAD);
 #undef CALL_GRAD
-    g_launches += 1;
+    if (err == cudaSuccess) g_launches += 1;
     return (int)err;
 }

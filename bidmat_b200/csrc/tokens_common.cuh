@@ -60,6 +60,9 @@ constexpr int kMostRows = 0x7fff0000;
 inline size_t dtype_size(int dtype) { return dtype == BIDMAT_B200_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == BIDMAT_B200_F32 || dtype == BIDMAT_B200_BF16 || dtype == BIDMAT_B200_F16; }
 
+// Finite, positive and not subnormal, so that 1.44 / temperature is a number.
+inline bool temperature_ok(float t) { return isfinite(t) && t >= 1.17549435e-38f; }
+
 // A dense operand: its leading dimension covers the rows, its address is aligned to its elements.
 inline bool dense_ok(const void *p, long long ld, int nrows, int dtype) {
     return p && ld >= nrows && (reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0;

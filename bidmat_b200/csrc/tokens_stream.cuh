@@ -175,14 +175,10 @@ __device__ __forceinline__ void copy16(void *smem, const void *p) {
     const unsigned dst = (unsigned)__cvta_generic_to_shared(smem);
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(p) : "memory");
 }
-__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-// All but the last PENDING groups have arrived.
-template <int PENDING> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 
 // The two halves of a cluster-wide barrier.
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive;" ::: "memory"); }
-// An arrival that orders no memory: the fence of the other form waits for every store before it.
-__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait;" ::: "memory"); }
 
 // A barrier in shared memory that counts arriving bytes, for values that other CTAs of the cluster send here.
@@ -362,13 +358,12 @@ template <typename T> struct Slice {
 #pragma unroll 4
         for (int i = tid; i < hi; i += THREADS, p += THREADS * N)
             if (i >= lo) copy16(kept + i, p);
-        copies_commit();
     }
     // Waits for them; partial vectors get -infinity where they are not the column's.
     template <int THREADS>
     __device__ __forceinline__ void arrive(uint4 *kept, const T *X, const T *end, const T *column, int rows) const {
         const int tid = threadIdx.x;
-        copies_wait<0>();
+        copies_wait();
         if ((head && tid == 0) || (tail && tid == (last & (THREADS - 1)))) {
             const Column<T> whole(column, rows);
             const bool one = head && tail && last == 0;

@@ -430,7 +430,8 @@ BIDMAT_B200_API int bidmat_b200_route_grad(int nrows, int ncols, int nnz, const 
  * entries per column (arrays as in bidmat_b200_route): the rows and the logits themselves, in descending
  * order, equal logits by ascending row; NaN counts as larger than any number, -0 as equal to 0.
  * lse (ncols values, may be NULL) receives log sum_v exp(X[v]/temperature) of every column.
- * 1 <= k <= BIDMAT_B200_TOP_MAX_K, k <= nrows; temperature is finite and > 0. */
+ * 1 <= k <= BIDMAT_B200_TOP_MAX_K, k <= nrows; temperature is a finite normal number > 0; nrows and
+ * ncols are at most 2^31 - 65536 here and in the functions below. */
 #define BIDMAT_B200_TOP_MAX_K 512
 BIDMAT_B200_API int bidmat_b200_top_logits(int nrows, int ncols, const void *X, long long ldx, int dtype, int k,
                                            float temperature, int *Sir, int *Sic, int *Sjc, float *Sdata, float *lse,
@@ -438,7 +439,7 @@ BIDMAT_B200_API int bidmat_b200_top_logits(int nrows, int ncols, const void *X, 
 
 /* Distillation: Kullback-Leibler divergence of a student's logits X(nrows x ncols) from a teacher's top
  * logits Z(nrows x ncols, sparse: Zir, Zjc, Zdata, any number of entries per column in any order), with
- * t = temperature and, per column,
+ * t = temperature (finite, normal, > 0) and, per column,
  *     p_i  = exp(z_i/t - Lt),  Lt = Zlse[column], or, with Zlse == NULL, the log-sum-exp of the column's
  *            entries z_i/t (p then sums to one over the entries),
  *     L    = log sum_v exp(X[v]/t),

@@ -145,6 +145,35 @@ def test_route_ties_and_near_ties(cuda_device, score, biased):
         check_route(z.astype(np.float32), "fp32", cuda_device, 8, score=score, bias=(0.5 - p[7]).astype(np.float32))
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("E,k", [(256, 8), (160, 6), (64, 3), (512, 8), (1024, 32), (256, 31)])
+def test_route_columns_in_bad_orders(cuda_device, dtype, E, k):
+    """Columns whose largest scores lie where few lanes have them, constant ones, and ones with fewer rows than picks."""
+    rng = np.random.default_rng(E + k)
+    x = rng.standard_normal((24, E))
+    x[0] = 0.0                                                  # a mixture before its first step
+    x[1] = np.round(x[1])
+    x[2] = np.linspace(-3, 3, E)
+    x[3] = np.linspace(3, -3, E)
+    for i, m in enumerate((4, 8, 16, 32, 64)):
+        x[4 + i, ::m] += 10.0
+    x[9, : E // 2] += 10.0
+    x[10, 8:16] += 10.0
+    x[11] = np.where(np.arange(E) % 2 == 0, 1.0, -1.0)
+    x[12, k - 1:] = -np.inf
+    x[13, :-1] = -np.inf
+    x[14] = -np.inf
+    x[15] = 1.0
+    x[15, 5] = 2.0
+    x[16] = np.repeat(rng.standard_normal(E // 4), 4)
+    bias = 0.1 * rng.standard_normal(E)
+    for b in (None, bias, np.zeros(E)):
+        for score in ("softmax", "sigmoid"):
+            check_route(x, dtype, cuda_device, k, score=score, bias=b)
+            check_route(x, dtype, cuda_device, k, score=score, bias=b, groups=8, topgroups=4, renorm=False)
+            check_route(x, dtype, cuda_device, k, score=score, bias=b, groups=4, topgroups=2, grouptop=1)
+
+
 def test_route_masks_infinities_and_nan(cuda_device):
     rng = np.random.default_rng(8)
     x = rng.standard_normal((40, 48)).astype(np.float32)

@@ -40,10 +40,12 @@ DISTILL_BOTH = dict(nrows=100, ncols=4, nnz=24, X=P, ldx=100, dtype=0, temperatu
                                 dict(Sjc=0), dict(Sdata=0), dict(dS=0), dict(ldx=80)]),
     (TOP, "top_logits", [dict(nrows=0), dict(nrows=9, ldx=9), dict(ncols=-1), dict(X=0), dict(X=P + 1), dict(ldx=99),
                          dict(dtype=4), dict(k=0), dict(k=513, nrows=1000, ldx=1000), dict(temperature=0.0),
-                         dict(temperature=-1.0), dict(temperature=NAN), dict(temperature=INF), dict(Sir=0), dict(Sic=0),
+                         dict(temperature=-1.0), dict(temperature=1e-39), dict(nrows=2147483647, ldx=2147483647),
+                         dict(temperature=NAN), dict(temperature=INF), dict(Sir=0), dict(Sic=0),
                          dict(Sjc=0), dict(Sdata=0), dict(ncols=2147483647)]),
     (DISTILL, "distill", [dict(nrows=0), dict(ncols=-1), dict(nnz=-1), dict(X=0), dict(X=P + 1), dict(ldx=99),
-                          dict(dtype=3), dict(temperature=0.0), dict(temperature=NAN), dict(Zir=0), dict(Zjc=0),
+                          dict(dtype=3), dict(temperature=0.0), dict(temperature=1e-39), dict(temperature=NAN),
+                          dict(nrows=2147483647, ldx=2147483647), dict(ncols=2147483647), dict(Zir=0), dict(Zjc=0),
                           dict(Zdata=0), dict(loss=0), dict(Xlse=0)]),
     (DISTILL_GRAD, "distill_grad", [dict(nrows=0), dict(ncols=-1), dict(nnz=-1), dict(X=0), dict(ldx=99), dict(dtype=3),
                                     dict(temperature=-2.0), dict(temperature=INF), dict(Zir=0), dict(Zjc=0),
