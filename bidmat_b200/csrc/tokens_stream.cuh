@@ -250,21 +250,24 @@ __device__ __forceinline__ float2 exp_pair(float a, float b, unsigned long long 
     return make_float2(exp2_fast(e.x), exp2_fast(e.y));
 }
 
-// top: the vector's maximum; it may be NaN if an element is.
-template <typename T> __device__ __forceinline__ void add_vector(SumExp &a, const uint4 &r, float top, float c) {
+// top: the vectors' maximum.
+template <typename T, int K> __device__ __forceinline__ void add_vectors(SumExp &a, const uint4 (&r)[K], float top, float c) {
     constexpr int N = Pack<T>::N;
     if (top > a.m) a.raise(top, c);
-    float v[N];
-    Pack<T>::unpack(r, v);
     const float ref = a.ref();
     const unsigned long long mr = pair(-ref, -ref), cc = pair(c, c);
-    unsigned long long acc = pair(0.f, 0.f);
+    unsigned long long acc[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-    for (int j = 0; j < N; j += 2) {
-        const float2 e = exp_pair(v[j], v[j + 1], mr, cc);
-        acc = add2(acc, pair(e.x, e.y));
+    for (int k = 0; k < K; k++) {
+        float v[N];
+        Pack<T>::unpack(r[k], v);
+#pragma unroll
+        for (int j = 0; j < N; j += 2) {
+            const float2 e = exp_pair(v[j], v[j + 1], mr, cc);
+            acc[(j >> 1) & 1] = add2(acc[(j >> 1) & 1], pair(e.x, e.y));
+        }
     }
-    const float2 e = unpair(acc);
+    const float2 e = unpair(add2(acc[0], acc[1]));
     a.s += e.x + e.y;
 }
 
@@ -308,18 +311,20 @@ __device__ __forceinline__ SumExp sum_exp_slice(const Column<T> &x, int v0, int 
         uint4 r[U];
 #pragma unroll
         for (int u = 0; u < U; u++) r[u] = x.load(i + u * THREADS);
+        float top = Pack<T>::max(r[0]);
 #pragma unroll
-        for (int u = 0; u < U; u++) add_vector<T>(a, r[u], Pack<T>::max(r[u]), c);
+        for (int u = 1; u < U; u++) top = fmaxf(top, Pack<T>::max(r[u]));
+        add_vectors<T, U>(a, r, top, c);
     }
     for (; i < f1; i += THREADS) {
-        const uint4 r = x.load(i);
-        add_vector<T>(a, r, Pack<T>::max(r), c);
+        const uint4 r[1] = {x.load(i)};
+        add_vectors<T, 1>(a, r, Pack<T>::max(r[0]), c);
     }
     if (threadIdx.x < 2) {
         const int p = x.partial((int)threadIdx.x, v0, v1);
         if (p >= 0) {
-            const uint4 r = x.load_partial(p);
-            add_vector<T>(a, r, Pack<T>::max(r), c);
+            const uint4 r[1] = {x.load_partial(p)};
+            add_vectors<T, 1>(a, r, Pack<T>::max(r[0]), c);
         }
     }
     return a;

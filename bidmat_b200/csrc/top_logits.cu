@@ -12,7 +12,7 @@
 //      round, so of equal values the later ones need not be looked at once there are k.
 //   3. In the end the parts of a cluster are put together in its first CTA; what the k-th largest entry leaves (k, or a
 //      few more) goes to the place that its rank gives.
-// Bound by memory with many long columns (131072 x 2048 bf16, k = 64: 176 us with the log-sum-exp, 124 us without, 82 us to read), by the chain of steps with few
+// Bound by memory with many long columns (131072 x 2048 bf16, k = 64: 163 us with the log-sum-exp, 120 us without, 82 us to read), by the chain of steps with few
 // (32768 x 1 fp32, k = 40: 9.3 us).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
 // CTAs spent most of their time on the bounds and on waiting for the cluster.
 #include <cuda_runtime.h>
@@ -41,7 +41,7 @@ struct TopArgs {
 constexpr int kTop = 256;                                   // threads
 constexpr int kRound = 4;                                   // vectors per thread and round
 constexpr int kSlack = 64;                                  // entries beyond k that a selection may leave
-constexpr int kDrain = 128;                                 // vectors set aside that are worth going through
+constexpr int kDrain = 192;                                  // vectors set aside that are worth going through
 constexpr int kBatch = kTop * 8;                            // values that are listed between two looks at the length
 constexpr int kList = kBatch + BIDMAT_B200_TOP_MAX_K + kSlack;
 
@@ -148,7 +148,7 @@ template <typename T> __device__ __noinline__ unsigned go_through(TopShared &sh,
     }
     __syncthreads();
     if (threadIdx.x == 0) sh.set_aside = 0;
-    if (sh.length >= 2 * k + 256) from = max(from, cut(sh, k));
+    if (sh.length >= 2 * k + 128) from = max(from, cut(sh, k));
     // later rows are larger: what equals the k-th of the list comes behind it
     return from == (Entry)(bound + 1) << 32 ? bound : key_of(from);
 }
@@ -193,10 +193,8 @@ __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int g
         for (int k = 0; k < kRound; k++) r[k] = next[k];
         if (r0 + step < v1) fetch(next, r0 + step);
 #pragma unroll
-        for (int k = 0; k < kRound; k++) {
-            top[k] = Pack<T>::max_nan(r[k]);
-            if (LSE) add_vector<T>(s, r[k], top[k], a.c);
-        }
+        for (int k = 0; k < kRound; k++) top[k] = Pack<T>::max_nan(r[k]);
+        if (LSE) add_vectors<T, kRound>(s, r, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.c);
         unsigned first = 0;
         if (r0 == v0) {
             // 16 bits of the k-th largest maximum are enough; what equals them is wanted in this round
@@ -285,7 +283,7 @@ __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int g
 }
 
 // A CTA per column, or as many as the machine holds at a time (three or four per SM): a second wave would cost more than a
-// CTA's longer way (100003 x 257 fp16: 32 us in one part, 43 us in three).
+// CTA's longer way (100003 x 257 fp16: 30 us in one part, 43 us in three).
 template <typename T> cudaError_t launch_top(const TopArgs &a, const void *X, cudaStream_t st) {
     const long long bytes = (long long)a.nrows * (long long)sizeof(T);
     const long long fill = 444 / a.ncols, worth = (bytes + 8191) / 8192;
