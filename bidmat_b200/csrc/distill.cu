@@ -268,7 +268,7 @@ struct DistillArgs {
 // entries' rows, which the other warps leave out when they write, and writes those itself.
 //   BOTH: the CTAs of a cluster have one column.  Every warp sums up its rows and sends (m, s) to every CTA.
 //   GRAD: the log-sum-exp is given; CTAs have nothing to do with one another.
-// CTAs are short-lived and five of them share an SM, so that one's loads overlap another's arithmetic and stores.
+// CTAs are short-lived and three to five of them share an SM, so that one's loads overlap another's arithmetic and stores.
 enum Mode { GRAD, BOTH };
 
 // The sum of what every warp of the cluster has sent here.
@@ -282,13 +282,13 @@ template <int W> __device__ __forceinline__ SumExp receive(unsigned long long *a
 }
 
 __device__ __forceinline__ void write_loss(const DistillArgs &a, long long col, const SumExp &s, const Entries &e, float w) {
-    const double L = s.m == -INFINITY ? (double)(s.s == 0.f ? -INFINITY : NAN) : s.m / (double)a.t + log((double)s.s);
+    const double L = s.log_sum(a.t, a.c);
     if (a.lse_out) a.lse_out[col] = (float)L;
     a.loss[col] = e.P == 0.0 ? 0.f : (float)((double)w * (e.cross + e.P * (L - e.lt)));
 }
 
 template <typename T, int THREADS, Mode MODE>
-__global__ void __launch_bounds__(THREADS + 32, THREADS == 256 ? 5 : 14)
+__global__ void __launch_bounds__(THREADS + 32, THREADS == 64 ? 14 : (MODE == GRAD ? 5 : 3))
 distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
     constexpr int N = Pack<T>::N, W = THREADS / 32;
     __shared__ float2 joined[MODE == GRAD ? 1 : 8 * W];         // (m, s) of every warp of the cluster
@@ -359,7 +359,7 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
         if (MODE == BOTH) {
             const SumExp s = receive<W>(&arrived, joined, l.parts * W, a.c);
             ref = s.ref();
-            qf = 1.f / s.s;
+            qf = (float)(1.0 / s.exact(a.c));
             if (part == 0 && lane == 0) write_loss(a, col, s, e, w);
         }
         const bool plain = (twice & 1) == 0;
@@ -382,25 +382,30 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
     }
 
     x.template arrive<THREADS>(kept, X, end, X + col * a.ldx, a.nrows);
-    float f, ref;
+    float f, ref, f_exact = 0.f;    // f_exact: relative to the reference itself
     if (MODE == BOTH) {
         SumExp s;
 #pragma unroll 4
         for (int i = tid; i < x.n; i += THREADS) s.m = fmaxf(s.m, Pack<T>::max(kept[i]));
-        const unsigned long long mr = pair(-s.ref(), -s.ref()), cc = pair(a.c, a.c);
-        unsigned long long acc = pair(0.f, 0.f);
+        const float k0 = __fmul_rn(s.ref(), a.c);
+        if (moderate(k0)) {
+            const unsigned long long cc = pair(a.c, a.c), mk = pair(-k0, -k0);
+            unsigned long long acc = pair(0.f, 0.f);
 #pragma unroll 2
-        for (int i = tid; i < x.n; i += THREADS) {
-            float v[N];
-            Pack<T>::unpack(kept[i], v);
+            for (int i = tid; i < x.n; i += THREADS) {
+                float v[N];
+                Pack<T>::unpack(kept[i], v);
 #pragma unroll
-            for (int j = 0; j < N; j += 2) {
-                const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
-                acc = add2(acc, pair(q.x, q.y));
+                for (int j = 0; j < N; j += 2) {
+                    const float2 q = exp_pair_from(v[j], v[j + 1], cc, mk);
+                    acc = add2(acc, pair(q.x, q.y));
+                }
             }
+            const float2 q = unpair(acc);
+            s.s = q.x + q.y;
+        } else {
+            for (int i = tid; i < x.n; i += THREADS) s.s += sum_of_differences<T>(kept[i], s.ref(), a.c);
         }
-        const float2 q = unpair(acc);
-        s.s = q.x + q.y;
         warp_join(s, a.c);
         cluster_wait();
         if (lane < l.parts) mail_send(&joined[part * W + (tid >> 5)], &arrived, lane, make_float2(s.m, s.s));
@@ -408,26 +413,14 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
         const SumExp sum = receive<W>(&arrived, joined, l.parts * W, a.c);
         ref = sum.ref();
         f = slope.x / sum.s;
+        f_exact = slope.x / (float)sum.exact(a.c);
     } else {
         __syncthreads();
         f = slope.x;
         ref = slope.y;
     }
     const bool zero = (twice & 2) != 0, wide = (reinterpret_cast<uintptr_t>(out) & 15) == 0;
-    const unsigned long long mr = pair(-ref, -ref), cc = pair(a.c, a.c), ff = pair(f, f);
-#pragma unroll 2
-    for (int i = tid; i < x.n; i += THREADS) {
-        float v[N];
-        Pack<T>::unpack(kept[i], v);
-#pragma unroll
-        for (int j = 0; j < N; j += 2) {
-            const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
-            const float2 y = unpair(mul2(pair(q.x, q.y), ff));
-            v[j] = y.x;
-            v[j + 1] = y.y;
-        }
-        uint4 y = Pack<T>::pack(v);
-        if (zero) y = make_uint4(0, 0, 0, 0);
+    auto store = [&](int i, const uint4 &y) {
         const unsigned skip = marks[i];
         if (wide && !skip) {
             store16(out + (long long)i * N, y);
@@ -435,6 +428,45 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
 #pragma unroll
             for (int j = 0; j < N; j++)
                 if (!((skip >> j) & 1u)) out[(long long)i * N + j] = reinterpret_cast<const T *>(&y)[j];
+        }
+    };
+    // exponents relative to the reference, for 16-bit gradients with the factor among them (its logarithm costs them nothing
+    // they could tell: 2^-24 of an exponent of 30 or so)
+    constexpr bool FOLD = sizeof(T) == 2;
+    const float k0 = __fmul_rn(ref, a.c), shift = FOLD ? k0 - log2f(fabsf(f)) : k0;
+    if (zero) {
+        for (int i = tid; i < x.n; i += THREADS) store(i, make_uint4(0, 0, 0, 0));
+    } else if (moderate(k0) && !(MODE == GRAD && !FOLD) && !(FOLD && f < 0.f)) {
+        const unsigned long long cc = pair(a.c, a.c), mk = pair(-shift, -shift), ff = pair(f, f);
+#pragma unroll 2
+        for (int i = tid; i < x.n; i += THREADS) {
+            float v[N];
+            Pack<T>::unpack(kept[i], v);
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                float2 y = exp_pair_from(v[j], v[j + 1], cc, mk);
+                if (!FOLD) y = unpair(mul2(pair(y.x, y.y), ff));
+                v[j] = y.x;
+                v[j + 1] = y.y;
+            }
+            store(i, Pack<T>::pack(v));
+        }
+    } else {
+        // differences first: references beyond 1e37, negative weights in 16 bits, fp32 gradients from a saved log-sum-exp
+        const float f1 = MODE == BOTH && moderate(k0) ? f_exact : f;
+        const unsigned long long mr = pair(-ref, -ref), cc = pair(a.c, a.c), ff = pair(f1, f1);
+#pragma unroll 2
+        for (int i = tid; i < x.n; i += THREADS) {
+            float v[N];
+            Pack<T>::unpack(kept[i], v);
+#pragma unroll
+            for (int j = 0; j < N; j += 2) {
+                const float2 q = exp_pair(v[j], v[j + 1], mr, cc);
+                const float2 y = unpair(mul2(pair(q.x, q.y), ff));
+                v[j] = y.x;
+                v[j + 1] = y.y;
+            }
+            store(i, Pack<T>::pack(v));
         }
     }
 }
@@ -495,7 +527,8 @@ distill_long_kernel(DistillArgs a, const T *X, T *dX) {
             write_zeros<T, kStream + 32>(x, out, v0, v1);
             return;
         }
-        const Slope g{a.t, a.c, w, s.ref(), (float)e.P * w / (a.t * s.s), 1.0 / s.s, e.lt, e.P};
+        const double sum = s.exact(a.c);
+        const Slope g{a.t, a.c, w, s.ref(), (float)e.P * w / (a.t * (float)sum), 1.0 / sum, e.lt, e.P};
         write_gradient<T, kStream + 32>(x, out, a.z, j0, j1, v0, v1, g, marks, &twice);
     }
 }
@@ -526,17 +559,20 @@ cudaError_t launch_long(const DistillArgs &a, int ncols, int size, const void *X
     return cudaLaunchKernelEx(&cfg, distill_long_kernel<T, GRADIENT>, a, (const T *)X, (T *)dX);
 }
 
-// Parts of 32 KB keep five CTAs on an SM; a cluster has at most 8 parts, so columns of up to 512 KB get larger ones, and
-// those beyond are read twice.  Where columns are few they are cut into more parts, to give every SM two CTAs.  Columns of
-// up to 8 KB have a small CTA each.
-constexpr long long kPartBytes = 32768, kMostPartBytes = 65536, kShortBytes = 8192;
+// Parts, 131072 x 2048 bf16.  BOTH: of 64 KB, three CTAs on an SM, 195 us; 32 KB and five CTAs 225 us, 48 KB and four 212 us,
+// 96 KB and two 221 us: with fewer parts fewer CTAs wait for one another.  GRAD: nobody waits, 32 KB and five CTAs.  A cluster has
+// at most 8 parts, so columns above 512 KB get parts of up to 96 KB and those above 768 KB are read twice.  Where columns
+// are few they are cut into more parts, to give every SM two CTAs.  Columns of up to 32 KB have CTAs of 96 threads
+// (8000 x 8192 bf16, BOTH: 83 us, 122 us with 288 threads).
+constexpr long long kGradBytes = 32768, kBothBytes = 65536, kMostPartBytes = 98304, kShortBytes = 32768;
 
 template <typename T, Mode MODE>
 cudaError_t launch_distill(const DistillArgs &a, int ncols, const void *X, void *dX, cudaStream_t st) {
     const long long nvec = most_vectors<T>(X, a.ldx, a.nrows, ncols), bytes = nvec * 16;
     const long long most = MODE == GRAD ? nvec : 8;
     const bool small = bytes <= kShortBytes;
-    long long parts = (bytes + kPartBytes - 1) / kPartBytes;
+    const long long part_bytes = MODE == GRAD ? kGradBytes : kBothBytes;
+    long long parts = (bytes + part_bytes - 1) / part_bytes;
     const long long fill = (296 + ncols - 1) / ncols, worth = (nvec + (small ? 63 : 255)) / (small ? 64 : 256);
     if (parts < fill) parts = fill < worth ? fill : worth;
     if (parts > most) parts = most;

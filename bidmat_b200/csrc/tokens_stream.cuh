@@ -5,9 +5,10 @@
 // the column; vector i holds the positions [i N, (i+1) N), N = 16 / sizeof(T).  Only the first and the last
 // vector can be partial; their elements are moved one by one, so nothing outside the column is touched.
 //
-// A thread keeps (m, s): the largest x so far and the sum of exp((x - m)/t) over its rows, taken as
-// 2^((x - m) c), c = log2(e)/t.  The difference comes first, so a column of the type's lowest value (a mask
-// that leaves nothing) neither overflows nor loses its uniform distribution.
+// A thread keeps (m, s): the largest x so far and the sum of 2^(x c - k) over its rows, c = log2(e)/t and k = m c as fp32
+// rounds it.  That takes one instruction for two differences, and k's rounding is made up for where the sum is used
+// (exact()).  Where m c is beyond 1e37 (a mask of the type's lowest value that leaves nothing, say) the differences
+// x - m come first instead, so that such a column neither overflows nor loses its uniform distribution.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -213,13 +214,31 @@ __device__ __forceinline__ bool mail_wait(unsigned long long *bar, unsigned pari
     return false;
 }
 
+// k of a maximum, and whether exponents are taken relative to it.
+__device__ __forceinline__ bool moderate(float k) { return fabsf(k) <= 1e37f; }
+// The exponent that brings a sum relative to m1 up to m2 >= m1.
+__device__ __forceinline__ float rise(float m1, float m2, float c) {
+    const float k1 = __fmul_rn(m1, c), k2 = __fmul_rn(m2, c);
+    return moderate(k1) && moderate(k2) ? k1 - k2 : (m1 - m2) * c;
+}
+
 struct SumExp {
     float m = -INFINITY, s = 0.f;
     // what is subtracted: m, or 0 while everything was -infinity (the sum is then 0)
     __device__ __forceinline__ float ref() const { return m == -INFINITY ? 0.f : m; }
     __device__ __forceinline__ void raise(float top, float c) {
-        s = s == 0.f ? 0.f : s * exp2_fast((m - top) * c);       // a NaN stays
+        s = s == 0.f ? 0.f : s * exp2_fast(rise(m, top, c));     // a NaN stays
         m = top;
+    }
+    // the sum of exp((x - m)/t)
+    __device__ __forceinline__ double exact(float c) const {
+        const float k = __fmul_rn(ref(), c);
+        return moderate(k) ? s * (1.0 - ((double)ref() * c - k) * kLn2) : (double)s;
+    }
+    // log sum exp(x/t)
+    __device__ __forceinline__ double log_sum(float t, float c) const {
+        if (m == -INFINITY) return s == 0.f ? -INFINITY : NAN;
+        return m / (double)t + log(exact(c));
     }
 };
 
@@ -244,40 +263,63 @@ __device__ __forceinline__ unsigned long long mul2(unsigned long long a, unsigne
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
 }
+__device__ __forceinline__ unsigned long long fma2(unsigned long long a, unsigned long long b, unsigned long long c) {
+    unsigned long long r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+// 2^(a c - k), 2^(b c - k)
+__device__ __forceinline__ float2 exp_pair_from(float a, float b, unsigned long long cc, unsigned long long minus_k) {
+    const float2 e = unpair(fma2(pair(a, b), cc, minus_k));
+    return make_float2(exp2_fast(e.x), exp2_fast(e.y));
+}
 // 2^((a - ref) c), 2^((b - ref) c)
 __device__ __forceinline__ float2 exp_pair(float a, float b, unsigned long long minus_ref, unsigned long long cc) {
     const float2 e = unpair(mul2(add2(pair(a, b), minus_ref), cc));
     return make_float2(exp2_fast(e.x), exp2_fast(e.y));
 }
 
+// The sum of 2^((x - ref) c) over a vector: for maxima that are not moderate.
+template <typename T> __device__ __noinline__ float sum_of_differences(const uint4 r, float ref, float c) {
+    constexpr int N = Pack<T>::N;
+    float v[N], sum = 0.f;
+    Pack<T>::unpack(r, v);
+    for (int j = 0; j < N; j++) sum += exp2_fast((v[j] - ref) * c);
+    return sum;
+}
+
 // top: the vectors' maximum.
 template <typename T, int K> __device__ __forceinline__ void add_vectors(SumExp &a, const uint4 (&r)[K], float top, float c) {
     constexpr int N = Pack<T>::N;
     if (top > a.m) a.raise(top, c);
-    const float ref = a.ref();
-    const unsigned long long mr = pair(-ref, -ref), cc = pair(c, c);
-    unsigned long long acc[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
+    const float ref = a.ref(), k0 = __fmul_rn(ref, c);
+    if (moderate(k0)) {
+        const unsigned long long cc = pair(c, c), mk = pair(-k0, -k0);
+        unsigned long long acc[2] = {pair(0.f, 0.f), pair(0.f, 0.f)};
 #pragma unroll
-    for (int k = 0; k < K; k++) {
-        float v[N];
-        Pack<T>::unpack(r[k], v);
+        for (int k = 0; k < K; k++) {
+            float v[N];
+            Pack<T>::unpack(r[k], v);
 #pragma unroll
-        for (int j = 0; j < N; j += 2) {
-            const float2 e = exp_pair(v[j], v[j + 1], mr, cc);
-            acc[(j >> 1) & 1] = add2(acc[(j >> 1) & 1], pair(e.x, e.y));
+            for (int j = 0; j < N; j += 2) {
+                const float2 e = exp_pair_from(v[j], v[j + 1], cc, mk);
+                acc[(j >> 1) & 1] = add2(acc[(j >> 1) & 1], pair(e.x, e.y));
+            }
         }
+        const float2 e = unpair(add2(acc[0], acc[1]));
+        a.s += e.x + e.y;
+    } else {
+#pragma unroll
+        for (int k = 0; k < K; k++) a.s += sum_of_differences<T>(r[k], ref, c);
     }
-    const float2 e = unpair(add2(acc[0], acc[1]));
-    a.s += e.x + e.y;
 }
 
-// Both partners of an exchange get the same bits: the smaller maximum is always brought up to the larger one.
 __device__ __forceinline__ void join(SumExp &a, float m, float s, float c) {
     if (m > a.m) {
         a.raise(m, c);
         a.s += s;
     } else {
-        a.s += s == 0.f ? 0.f : (m == a.m ? s : s * exp2_fast((m - a.m) * c));
+        a.s += s == 0.f ? 0.f : (m == a.m ? s : s * exp2_fast(rise(m, a.m, c)));
     }
 }
 // Largest of the warp's values (none of them NaN).
@@ -289,7 +331,7 @@ __device__ __forceinline__ float warp_top(float v) {
 // The same result in every lane: the sums are brought up to the largest maximum, then added.
 __device__ __forceinline__ void warp_join(SumExp &a, float c) {
     const float m = warp_top(a.m);
-    a.s = a.m == m || a.s == 0.f ? a.s : a.s * exp2_fast((a.m - m) * c);
+    a.s = a.m == m || a.s == 0.f ? a.s : a.s * exp2_fast(rise(a.m, m, c));
     a.m = m;
     a.s = warp_sum(a.s);
 }
@@ -360,9 +402,11 @@ template <typename T> struct Slice {
     template <int THREADS> __device__ __forceinline__ void copy(uint4 *kept, const T *X, const T *end) const {
         const int tid = threadIdx.x, lo = head && !whole_head(X), hi = n - (tail && !whole_tail(end));
         const T *p = base + (long long)tid * N;
+        uint4 *to = kept + tid;
+        int i = tid;
+        if (i < lo) { i += THREADS; p += THREADS * N; to += THREADS; }
 #pragma unroll 4
-        for (int i = tid; i < hi; i += THREADS, p += THREADS * N)
-            if (i >= lo) copy16(kept + i, p);
+        for (; i < hi; i += THREADS, p += THREADS * N, to += THREADS) copy16(to, p);
     }
     // Waits for them; partial vectors get -infinity where they are not the column's.
     template <int THREADS>
