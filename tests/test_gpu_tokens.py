@@ -435,6 +435,46 @@ def test_distill_sizes_and_types(cuda_device, dtype, V, T, k):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("tau", [0.01, 0.3, 7.0, 500.0])
+@pytest.mark.parametrize("V", [300, 20000, 70000])
+def test_distill_temperatures_and_signs(cuda_device, dtype, tau, V):
+    """Sharp and flat distributions, weights of both signs."""
+    rng = np.random.default_rng(V)
+    jc, ir, z = teacher(rng, V, [20, 1, 40])
+    x = 2.0 * rng.standard_normal((3, V))
+    for t in range(3):
+        x[t, ir[jc[t]:jc[t + 1]]] = z[jc[t]:jc[t + 1]] + 0.2 * rng.standard_normal(jc[t + 1] - jc[t])
+    check_distill(x, jc, ir, z, dtype, cuda_device, tau=tau, weights=np.float32([-tau, 0.5 * tau, -3.0 * tau]))
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+def test_distill_of_lowest_values_and_large_ones(cuda_device, dtype):
+    """Columns masked with the lowest value, wholly or all but one row, and logits near the largest number: the
+    distribution is the one of the differences."""
+    V = 9000
+    low = float(np.finfo(np.float32).min) if dtype == "fp32" else -3.3e38
+    x = np.full((4, V), low)
+    x[1, 17] = 0.0
+    x[2] = 3.0e38 if dtype == "fp32" else 2.6e38
+    x[3] = np.linspace(-1, 1, V)
+    jc, ir, z = np.arange(0, 41, 10), np.tile(np.arange(10), 4).astype(np.int32), np.linspace(0, 1, 40).astype(np.float32)
+    X = dense(x, dtype, cuda_device)
+    Z = sparse(V, 4, jc, ir, z, cuda_device)
+    loss, L = tokens.distill(X, Z)
+    _, dX = tokens.distillWithGrad(X, Z)
+    # from the differences: next to 3e38 a log-sum-exp loses its logarithm in 64 bits as well
+    xs = host(X.t)
+    d = np.exp(xs - xs.max(1, keepdims=True))
+    want = d / d.sum(1, keepdims=True)
+    for t in range(4):
+        p = np.exp(z[jc[t]:jc[t + 1]].astype(np.float64))
+        want[t, :10] -= p / p.sum()
+    lse = xs.max(1) + np.log(d.sum(1))
+    close(host(L.t)[:, 0], lse, 4 * U * np.abs(lse) + 64 * U, "log-sum-exp")
+    close(host(dX.t), want, (HALF[dtype] + 64 * U) * np.abs(want) + 64 * U / 10, "gradient")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("V,T,k", [(5, 3, 5), (999, 40, 64), (70001, 3, 700), (300007, 2, 5)])
 def test_distill_gradient_in_place(cuda_device, dtype, V, T, k):
     rng = np.random.default_rng(V)
