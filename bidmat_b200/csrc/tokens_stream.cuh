@@ -3,7 +3,8 @@
 // A column of V elements starts at any element: it is treated as a row of 16-byte vectors from the aligned
 // address at or below its first element.  Position u = row + shift, shift = elements between that address and
 // the column; vector i holds the positions [i N, (i+1) N), N = 16 / sizeof(T).  Only the first and the last
-// vector can be partial; their elements are moved one by one, so nothing outside the column is touched.
+// vector can be partial.  They are read one element at a time, or whole where their other elements belong to the matrix as
+// well (between its first element and its last), and written one element at a time.
 //
 // A thread keeps (m, s): the largest x so far and the sum of 2^(x c - k) over its rows, c = log2(e)/t and k = m c as fp32
 // rounds it.  That takes one instruction for two differences, and k's rounding is made up for where the sum is used
