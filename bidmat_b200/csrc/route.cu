@@ -41,7 +41,7 @@ __device__ __forceinline__ void warp_best(double &key, int &row) {
 // The same for a column of which only the rows with an fp32 key of `cut` or more come into question: one row per lane.
 // False if there are more than 32 of them, or fewer than k.
 template <typename T>
-__device__ __noinline__ bool route_few(const RouteArgs &a, const T *__restrict__ x, const float *__restrict__ bias, long long c, float cut,
+__device__ __noinline__ bool route_few(const RouteArgs a, const T *__restrict__ x, const float *__restrict__ bias, long long c, float cut,
                                        const float *val, int *rows) {
     const int lane = threadIdx.x & 31;
     int n = 0;
@@ -91,7 +91,7 @@ __device__ __noinline__ bool route_few(const RouteArgs &a, const T *__restrict__
 // One column by one warp with everything that is compared in 64 bits.  val: nrows floats, rank: nrows + ngroups
 // doubles of shared memory.  groups: choose the groups as well; else val is -infinity where a row is out of the running.
 template <typename T>
-__device__ __noinline__ void route_exact(const RouteArgs &a, const T *__restrict__ x, const float *__restrict__ bias, long long c,
+__device__ __noinline__ void route_exact(const RouteArgs a, const T *__restrict__ x, const float *__restrict__ bias, long long c,
                                          bool groups, float *val, double *rank) {
     const int lane = threadIdx.x & 31;
     double *gval = rank + a.nrows;                  // rank: s + bias, -inf where out of the running
@@ -236,7 +236,7 @@ __device__ __forceinline__ float key_of(Entry e) { return order_value((unsigned)
 
 // G lanes have a column, each every G-th of its rows.  The (k+1)-th largest of the lanes' maxima is a bound that k + 1
 // rows reach; few more do, so the rows that reach it are listed and each is ranked by counting the ones before it.
-// (Sorted lists in the lanes' registers, joined by exchanges, took 36 and 47 us for the 256 x 4096 and 160 x 65537 below.)
+// (Sorted lists in the lanes' registers, joined by exchanges, took 36 and 47 us for 256 x 4096 fp32 with bias and groups and for 160 x 65537 bf16 with groups, this 10 and 36 us.)
 //
 // Where the order is that of scores plus bias, or of groups by their scores, it is found in fp32 first.  A sigmoid
 // s = 1/(1 + e) is then off by at most s (1 - s) (2^-22 + |x| 2^-23) + 1.5 s 2^-23 < 2^-22 (the exponential, the sum and the

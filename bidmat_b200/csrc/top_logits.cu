@@ -6,14 +6,16 @@
 //      largest of the groups' maxima is a value that k of the round's values reach, so nothing below it is among the
 //      column's k largest.  And it is tight: in no particular order, of 8192 values in 256 groups about 70 reach it for
 //      k = 64.
-//   2. A vector whose largest value is above the bound is set aside, which costs the others one comparison.  At the
-//      end of a round the vectors set aside are gone through by all threads, element by element, and what is above the
-//      bound is listed.  When the list has grown, its k-th largest entry becomes the bound.  Rows ascend from round to
-//      round, so of equal values the later ones need not be looked at once there are k.
+//   2. A vector whose largest value is above the bound is set aside, which costs the others one comparison.  Every few
+//      rounds the vectors set aside are gone through by all threads, element by element, and what is above the bound is
+//      listed.  (Rounds that set aside more than there is room for are repeated one by one.)  When the list has grown, its
+//      k-th largest entry becomes the bound.  Rows ascend from round to round, so of equal values the later ones need not
+//      be looked at once there are k.
 //   3. In the end the parts of a cluster are put together in its first CTA; what the k-th largest entry leaves (k, or a
 //      few more) goes to the place that its rank gives.
-// Bound by memory with many long columns (131072 x 2048 bf16, k = 64: 163 us with the log-sum-exp, 120 us without, 82 us to read), by the chain of steps with few
-// (32768 x 1 fp32, k = 40: 9.3 us).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
+// With many long columns the exponentials of the log-sum-exp and the steps between the rounds share the time with the
+// reading (131072 x 2048 bf16, k = 64: 159 us with the log-sum-exp, 112 us without, 82 us to read), with few columns the chain
+// of the steps counts (32768 x 1 fp32, k = 40: 9.2 us).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
 // CTAs spent most of their time on the bounds and on waiting for the cluster.
 #include <cuda_runtime.h>
 
@@ -41,14 +43,13 @@ struct TopArgs {
 constexpr int kTop = 256;                                   // threads
 constexpr int kRound = 4;                                   // vectors per thread and round
 constexpr int kSlack = 64;                                  // entries beyond k that a selection may leave
-constexpr int kDrain = 192;                                  // vectors set aside that are worth going through
-constexpr int kBatch = kTop * 8;                            // values that are listed between two looks at the length
+constexpr int kBatch = kTop * 4;                            // values that are listed between two looks at the length
 constexpr int kList = kBatch + BIDMAT_B200_TOP_MAX_K + kSlack;
 
 struct TopShared {
     Entry list[kList];
-    uint4 aside[kTop * kRound + kDrain];
-    int aside_at[kTop * kRound + kDrain];
+    uint4 aside[kTop * kRound];
+    int aside_at[kTop * kRound];
     unsigned hist[256];
     float2 sums[kTop / 32];
     int length, set_aside;
@@ -56,7 +57,9 @@ struct TopShared {
 };
 
 // One of the at most two vectors of a column that are not the column's alone.
-template <typename T> __device__ __noinline__ uint4 partial_vector(const Column<T> &x, int i) { return x.load_partial(i); }
+template <typename T> __device__ __noinline__ uint4 partial_vector(const T *column, int rows, int i) {
+    return Column<T>(column, rows).load_partial(i);
+}
 
 // The largest b = d 2^shift that at least k of the list's n entries reach, for the first shift from 56 down in steps of
 // 8 to `last` with which no more than k + kSlack do; how many reach it.  By the whole CTA, k <= n.
@@ -153,9 +156,61 @@ template <typename T> __device__ __noinline__ unsigned go_through(TopShared &sh,
     return from == (Entry)(bound + 1) << 32 ? bound : key_of(from);
 }
 
+// A bound as a float, of which NaN wants everything; 0x7fffffff, the key below zero's, would be the other zero.
+__device__ __forceinline__ float limit_of(unsigned key) { return order_value(key == 0x7fffffffu ? key - 1 : key); }
+
+// This thread's vectors of the round that starts at r0, -infinity behind v1.
+template <typename T>
+__device__ __forceinline__ void read_round(const Column<T> &x, int f0, int f1, int v1, int r0, uint4 (&r)[kRound]) {
+    constexpr int N = Pack<T>::N;
+    if (r0 >= f0 && r0 + kTop * kRound <= f1) {
+        const T *p = x.base + (long long)(r0 + (int)threadIdx.x) * N;
+#pragma unroll
+        for (int k = 0; k < kRound; k++) r[k] = load16(p + k * kTop * N);
+    } else {
+#pragma unroll
+        for (int k = 0; k < kRound; k++) {
+            const int i = r0 + (int)threadIdx.x + k * kTop;
+            r[k] = i >= f0 && i < f1 ? x.load(i) : (i < v1 ? partial_vector(x.base + x.shift, x.rows, i) : Pack<T>::lowest());
+        }
+    }
+}
+
+// Sets aside what may be above the limit, as far as there is room.
+__device__ __forceinline__ void set_aside(TopShared &sh, const uint4 (&r)[kRound], const float (&top)[kRound], float limit, int r0, int v1) {
+#pragma unroll
+    for (int k = 0; k < kRound; k++)
+        if (!(top[k] <= limit) && (r0 + kTop * kRound <= v1 || r0 + (int)threadIdx.x + k * kTop < v1)) {
+            const int at = atomicAdd(&sh.set_aside, 1);
+            if (at < kTop * kRound) {
+                sh.aside[at] = r[k];
+                sh.aside_at[at] = r0 + (int)threadIdx.x + k * kTop;
+            }
+        }
+}
+
+// The rounds from r0 to r1 once more, one at a time, because more had to be set aside than there was room for.
+template <typename T>
+__device__ __noinline__ unsigned repeat(TopShared &sh, const T *column, int rows, int f0, int f1, int v1, int r0, int r1, int k, unsigned bound) {
+    const Column<T> x(column, rows);
+    for (; r0 < r1; r0 += kTop * kRound) {
+        __syncthreads();
+        if (threadIdx.x == 0) sh.set_aside = 0;
+        __syncthreads();
+        uint4 r[kRound];
+        float top[kRound];
+        read_round(x, f0, f1, v1, r0, r);
+#pragma unroll
+        for (int i = 0; i < kRound; i++) top[i] = Pack<T>::max_nan(r[i]);
+        set_aside(sh, r, top, limit_of(bound), r0, v1);
+        __syncthreads();
+        bound = go_through<T>(sh, -x.shift, x.rows, k, bound);
+    }
+    return bound;
+}
+
 template <typename T, bool LSE>
 __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int groups, const T *X) {
-    constexpr int N = Pack<T>::N;
     __shared__ TopShared sh;
     cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, part = (int)cluster.block_rank(), parts = (int)cluster.num_blocks();
@@ -166,67 +221,51 @@ __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int g
     const int row0 = -x.shift;                                  // row of position 0
     if (tid == 0) sh.length = sh.set_aside = 0;
     unsigned bound = 0;                                         // values with a larger key are wanted
-    // as a float, of which NaN wants everything; 0x7fffffff, the key below zero's, would be the other zero
-    auto limit_of = [](unsigned key) { return order_value(key == 0x7fffffffu ? key - 1 : key); };
     float limit = limit_of(bound);
     SumExp s;
     const int step = kTop * kRound, f0 = max(v0, x.full0), f1 = min(v1, x.full1);
-    auto fetch = [&](uint4 (&r)[kRound], int r0) {
-        if (r0 >= f0 && r0 + step <= f1) {
-            const T *p = x.base + (long long)(r0 + tid) * N;
-#pragma unroll
-            for (int k = 0; k < kRound; k++) r[k] = load16(p + k * kTop * N);
-        } else {
-#pragma unroll
-            for (int k = 0; k < kRound; k++) {
-                const int i = r0 + tid + k * kTop;
-                r[k] = i >= f0 && i < f1 ? x.load(i) : (i < v1 ? partial_vector(x, i) : Pack<T>::lowest());
-            }
-        }
-    };
+    // Rounds between two barriers: one at first, then as many as are likely to find room for what they set aside.
+    const int block = a.k <= 128 ? 4 : (a.k <= 256 ? 2 : 1);
     uint4 next[kRound];
-    if (v0 < v1) fetch(next, v0);
-    for (int r0 = v0; r0 < v1; r0 += step) {
-        uint4 r[kRound];
-        float top[kRound];
-#pragma unroll
-        for (int k = 0; k < kRound; k++) r[k] = next[k];
-        if (r0 + step < v1) fetch(next, r0 + step);
-#pragma unroll
-        for (int k = 0; k < kRound; k++) top[k] = Pack<T>::max_nan(r[k]);
-        if (LSE) add_vectors<T, kRound>(s, r, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.c);
+    if (v0 < v1) read_round(x, f0, f1, v1, v0, next);
+    for (int b0 = v0; b0 < v1;) {
+        const int b1 = min(v1, b0 + (b0 == v0 ? step : block * step));
         unsigned first = 0;
-        if (r0 == v0) {
-            // 16 bits of the k-th largest maximum are enough; what equals them is wanted in this round
-            if (groups == kTop) {
-                sh.list[tid] = (Entry)order_key(larger_nan(larger_nan(top[0], top[1]), larger_nan(top[2], top[3]))) << 32;
-            } else {
+        for (int r0 = b0; r0 < b1; r0 += step) {
+            uint4 r[kRound];
+            float top[kRound];
 #pragma unroll
-                for (int k = 0; k < kRound; k++) sh.list[tid + k * kTop] = (Entry)order_key(top[k]) << 32;
-            }
-            __syncthreads();
-            int reach;
-            first = key_of(select(sh, groups, a.k, 48, &reach));
-            // groups of nothing but -infinity, or of nothing at all, give no bound
-            bound = first > order_key(-INFINITY) ? first - 1 : 0;
-            limit = limit_of(bound);
-        }
-        int at = 0;
+            for (int k = 0; k < kRound; k++) r[k] = next[k];
+            if (r0 + step < v1) read_round(x, f0, f1, v1, r0 + step, next);
 #pragma unroll
-        for (int k = 0; k < kRound; k++)
-            if (!(top[k] <= limit) && (r0 + step <= v1 || r0 + tid + k * kTop < v1)) {
-                at = atomicAdd(&sh.set_aside, 1);
-                sh.aside[at] = r[k];
-                sh.aside_at[at] = r0 + tid + k * kTop;
+            for (int k = 0; k < kRound; k++) top[k] = Pack<T>::max_nan(r[k]);
+            if (LSE) add_vectors<T, kRound>(s, r, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.c);
+            if (r0 == v0) {
+                // 16 bits of the k-th largest maximum are enough; what equals them is wanted in this round
+                if (groups == kTop) {
+                    sh.list[tid] = (Entry)order_key(larger_nan(larger_nan(top[0], top[1]), larger_nan(top[2], top[3]))) << 32;
+                } else {
+#pragma unroll
+                    for (int k = 0; k < kRound; k++) sh.list[tid + k * kTop] = (Entry)order_key(top[k]) << 32;
+                }
+                __syncthreads();
+                int reach;
+                first = key_of(select(sh, groups, a.k, 48, &reach));
+                // groups of nothing but -infinity, or of nothing at all, give no bound
+                bound = first > order_key(-INFINITY) ? first - 1 : 0;
+                limit = limit_of(bound);
             }
-        // one barrier per round; the bound changes with what is gone through only
-        if (__syncthreads_or(at + 1 >= kDrain || r0 == v0 || r0 + step >= v1)) {
-            const unsigned before = bound;
-            bound = go_through<T>(sh, row0, a.nrows, a.k, bound);
-            if (r0 == v0 && before > 0) bound = max(bound, first);
-            limit = limit_of(bound);
-            __syncthreads();
+            set_aside(sh, r, top, limit, r0, v1);
         }
+        __syncthreads();
+        const int aside = sh.set_aside;
+        const unsigned before = bound;
+        if (aside > kTop * kRound) bound = repeat(sh, x.base + x.shift, x.rows, f0, f1, v1, b0, b1, a.k, bound);
+        else if (aside > 0) bound = go_through<T>(sh, row0, a.nrows, a.k, bound);
+        if (b0 == v0 && before > 0) bound = max(bound, first);
+        limit = limit_of(bound);
+        __syncthreads();
+        b0 = b1;
     }
     if (LSE) {
         warp_join(s, a.c);
@@ -280,7 +319,7 @@ __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int g
 }
 
 // A CTA per column, or as many as the machine holds at a time (three or four per SM): a second wave would cost more than a
-// CTA's longer way (100003 x 257 fp16: 30 us in one part, 43 us in three).
+// CTA's longer way (100003 x 257 fp16: 28 us in one part, 43 us in three).
 template <typename T> cudaError_t launch_top(const TopArgs &a, const void *X, cudaStream_t st) {
     const long long bytes = (long long)a.nrows * (long long)sizeof(T);
     const long long fill = 444 / a.ncols, worth = (bytes + 8191) / 8192;
