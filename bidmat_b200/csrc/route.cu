@@ -236,7 +236,8 @@ __device__ __forceinline__ float key_of(Entry e) { return order_value((unsigned)
 
 // G lanes have a column, each every G-th of its rows.  The (k+1)-th largest of the lanes' maxima is a bound that k + 1
 // rows reach; few more do, so the rows that reach it are listed and each is ranked by counting the ones before it.
-// (Sorted lists in the lanes' registers, joined by exchanges, took 36 and 47 us for 256 x 4096 fp32 with bias and groups and for 160 x 65537 bf16 with groups, this 10 and 36 us.)
+// (256 x 4096 fp32 with bias and groups: 10 us, 36 us with sorted lists in the lanes' registers that are joined by exchanges;
+// 160 x 65537 bf16 with groups: 36 and 47 us.)
 //
 // Where the order is that of scores plus bias, or of groups by their scores, it is found in fp32 first.  A sigmoid
 // s = 1/(1 + e) is then off by at most s (1 - s) (2^-22 + |x| 2^-23) + 1.5 s 2^-23 < 2^-22 (the exponential, the sum and the
@@ -663,7 +664,7 @@ route_grad_kernel(RouteArgs a, int nnz, const T *X, const int *__restrict__ Sir,
         for (int i = sub; i * 4 < a.nrows; i += G) *reinterpret_cast<float4 *>(col + i * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncwarp();
-    const float back = a.renorm ? d / a.scale : 0.f;
+    const float back = a.renorm ? d * (1.f / a.scale) : 0.f;
     for (int j = j0; __any_sync(0xffffffffu, j < j1); j += G) {
         const bool have = j + sub < j1;
         const int row = have ? Sir[j + sub] : -1;
