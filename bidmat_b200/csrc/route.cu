@@ -236,7 +236,7 @@ __device__ __forceinline__ float key_of(Entry e) { return order_value((unsigned)
 
 // G lanes have a column, each every G-th of its rows.  The (k+1)-th largest of the lanes' maxima is a bound that k + 1
 // rows reach; few more do, so the rows that reach it are listed and each is ranked by counting the ones before it.
-// (256 x 4096 fp32 with bias and groups: 10 us, 36 us with sorted lists in the lanes' registers that are joined by exchanges;
+// (256 x 4096 fp32 with bias and groups: 9.2 us, 36 us with sorted lists in the lanes' registers that are joined by exchanges;
 // 160 x 65537 bf16 with groups: 36 and 47 us.)
 //
 // Where the order is that of scores plus bias, or of groups by their scores, it is found in fp32 first.  A sigmoid
@@ -252,7 +252,7 @@ __device__ __forceinline__ bool near(float a, float b, float within) {
 }
 
 template <typename T, int G, bool BIAS>
-__global__ void __launch_bounds__(kRouteWarps * 32)
+__global__ void __launch_bounds__(kRouteWarps * 32, 8)
 route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bias) {
     constexpr int C = 32 / G;                       // columns per warp
     constexpr int L = kListed * G, P = kListed;     // rows that can be listed, per column and per lane
@@ -341,22 +341,31 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     __syncwarp();
     bool again = false, groups_again = false;       // two neighbours too close
     if (a.ngroups > 1) {
-        // a lane takes whole groups; where their sizes would meet in one bank it begins each at another row than its neighbours
-        const int size = a.gsize;
-        auto first_of = [&](int g) { return (size & 7) ? 0 : (g < size ? g : g % size); };
+        // a lane takes whole groups, four rows at once where that divides them; groups that would meet in one bank are begun at
+        // another place in every lane
+        const int size = a.gsize, four = (size & 3) ? 0 : size / 4;
+        auto first_of = [&](int g) { return (size & 31) ? 0 : g % four; };
         for (int g = sub; g < a.ngroups; g += G) {
             float b1 = -INFINITY, b2 = -INFINITY;
-            const float *member = val + g * size;
             auto add = [&](float v) {
                 if (!BIAS && group_scores && v > -INFINITY) v = quick_score(v);
                 b2 = fmaxf(b2, fminf(b1, v));
                 b1 = fmaxf(b1, v);
             };
-            const int turn = first_of(g);
-#pragma unroll 4
-            for (int i = turn; i < size; i++) add(member[i]);
-#pragma unroll 4
-            for (int i = 0; i < turn; i++) add(member[i]);
+            if (four) {
+                const float4 *member = reinterpret_cast<const float4 *>(val) + g * four;
+                const int turn = first_of(g);
+                for (int i = turn, left = four; left > 0; left--) {
+                    const float4 v = member[i];
+                    add(v.x);
+                    add(v.y);
+                    add(v.z);
+                    add(v.w);
+                    if (++i == four) i = 0;
+                }
+            } else {
+                for (int i = 0; i < size; i++) add(val[g * size + i]);
+            }
             gval[g] = a.grouptop == 2 && b2 > -INFINITY ? b1 + b2 : b1;
         }
         __syncwarp();
@@ -383,12 +392,16 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         n = 0;
         for (int g = sub; g < a.ngroups; g += G, n++) {
             if (!((drop >> (n & 31)) & 1u)) continue;
-            float *member = val + g * size;
-            const int turn = first_of(g);
-#pragma unroll 4
-            for (int i = turn; i < size; i++) member[i] = -INFINITY;
-#pragma unroll 4
-            for (int i = 0; i < turn; i++) member[i] = -INFINITY;
+            if (four) {
+                float4 *member = reinterpret_cast<float4 *>(val) + g * four;
+                const int turn = first_of(g);
+                for (int i = turn, left = four; left > 0; left--) {
+                    member[i] = make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+                    if (++i == four) i = 0;
+                }
+            } else {
+                for (int i = 0; i < size; i++) val[g * size + i] = -INFINITY;
+            }
         }
         __syncwarp();
     }
