@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int g
             for (int k = 0; k < kRound; k++) top[k] = Pack<T>::max_nan(r[k]);
             if (LSE) add_vectors<T, kRound>(s, r, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])), a.c);
             if (r0 == v0) {
-                // 16 bits of the k-th largest maximum are enough; what equals them is wanted in this round
+                // 16 bits of the k-th largest maximum are enough; what equals them is wanted here
                 if (groups == kTop) {
                     sh.list[tid] = (Entry)order_key(larger_nan(larger_nan(top[0], top[1]), larger_nan(top[2], top[3]))) << 32;
                 } else {

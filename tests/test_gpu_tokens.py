@@ -416,7 +416,7 @@ def check_distill(x, jc, ir, z, dtype, device, tau=1.0, tlse=None, weights=None,
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
 @pytest.mark.parametrize("V,T,k", [(1, 1, 1), (3, 2, 3), (65, 7, 20), (1000, 3, 64), (1024, 2, 1000), (8192, 16, 20), (40001, 3, 100),
-                                   (65536, 2, 64), (131072, 2, 64), (100003, 5, 7), (300007, 2, 50)])
+                                   (65536, 2, 64), (131072, 2, 64), (100003, 5, 7), (300007, 2, 50), (500009, 2, 60)])
 def test_distill_sizes_and_types(cuda_device, dtype, V, T, k):
     rng = np.random.default_rng(V + 7 * T)
     counts = rng.integers(0, k + 1, T)
@@ -475,7 +475,7 @@ def test_distill_of_lowest_values_and_large_ones(cuda_device, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
-@pytest.mark.parametrize("V,T,k", [(5, 3, 5), (999, 40, 64), (70001, 3, 700), (300007, 2, 5)])
+@pytest.mark.parametrize("V,T,k", [(5, 3, 5), (999, 40, 64), (70001, 3, 700), (300007, 2, 5), (400003, 3, 300)])
 def test_distill_gradient_in_place(cuda_device, dtype, V, T, k):
     rng = np.random.default_rng(V)
     jc, ir, z = teacher(rng, V, rng.integers(0, k + 1, T))
