@@ -420,23 +420,26 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         }
         if (e < 4 * quads) top0 = fmaxf(top0, val[e]);
     }
-    if (!two) top0 = fmaxf(top0, top1);
-    int place0 = two && top1 > top0, place1 = top0 >= top1;
+    float bound = -INFINITY;                        // so few rows that all of them can be listed
+    if (a.nrows > 2 * G) {
+        if (!two) top0 = fmaxf(top0, top1);
+        int place0 = two && top1 > top0, place1 = top0 >= top1;
 #pragma unroll
-    for (int o = 1; o < G; o++) {
-        const int from = (sub + o) & (G - 1);
-        const float t0 = __shfl_sync(0xffffffffu, top0, from, G);
-        place0 += from < sub ? t0 >= top0 : t0 > top0;
-        if (two) {
-            const float t1 = __shfl_sync(0xffffffffu, top1, from, G);
-            place0 += from < sub ? t1 >= top0 : t1 > top0;
-            place1 += from < sub ? (t0 >= top1) + (t1 >= top1) : (t0 > top1) + (t1 > top1);
+        for (int o = 1; o < G; o++) {
+            const int from = (sub + o) & (G - 1);
+            const float t0 = __shfl_sync(0xffffffffu, top0, from, G);
+            place0 += from < sub ? t0 >= top0 : t0 > top0;
+            if (two) {
+                const float t1 = __shfl_sync(0xffffffffu, top1, from, G);
+                place0 += from < sub ? t1 >= top0 : t1 > top0;
+                place1 += from < sub ? (t0 >= top1) + (t1 >= top1) : (t0 > top1) + (t1 > top1);
+            }
         }
+        const int kth = min(a.k, two ? 2 * G - 1 : G - 1);
+        const unsigned who0 = __ballot_sync(0xffffffffu, place0 == kth) & mine, who1 = __ballot_sync(0xffffffffu, two && place1 == kth) & mine;
+        const float bound0 = __shfl_sync(0xffffffffu, top0, who0 ? __ffs(who0) - 1 : 0), bound1 = __shfl_sync(0xffffffffu, top1, who1 ? __ffs(who1) - 1 : 0);
+        bound = who0 ? bound0 : bound1;
     }
-    const int kth = min(a.k, two ? 2 * G - 1 : G - 1);
-    const unsigned who0 = __ballot_sync(0xffffffffu, place0 == kth) & mine, who1 = __ballot_sync(0xffffffffu, two && place1 == kth) & mine;
-    const float bound0 = __shfl_sync(0xffffffffu, top0, who0 ? __ffs(who0) - 1 : 0), bound1 = __shfl_sync(0xffffffffu, top1, who1 ? __ffs(who1) - 1 : 0);
-    const float bound = who0 ? bound0 : bound1;
     // the rows that reach it
     // bit 4 i + j of the mask: row 4 (sub + G i) + j
     unsigned mask = 0;
@@ -734,10 +737,12 @@ cudaError_t launch_route_as(RouteArgs a, const void *X, const float *bias, cudaS
     return cudaGetLastError();
 }
 
-// Eight lanes per column where each then has no more than 32 rows and one pick, a whole warp for more.
+// Eight or sixteen lanes per column where each then has no more than 32 rows and one pick, a whole warp for more.
 template <typename T> cudaError_t launch_route(const RouteArgs &a, const void *X, const float *bias, cudaStream_t st) {
     if (a.nrows <= 256 && a.k <= 8)
         return bias ? launch_route_as<T, 8, true>(a, X, bias, st) : launch_route_as<T, 8, false>(a, X, bias, st);
+    if (a.nrows <= 512 && a.k <= 16)
+        return bias ? launch_route_as<T, 16, true>(a, X, bias, st) : launch_route_as<T, 16, false>(a, X, bias, st);
     return bias ? launch_route_as<T, 32, true>(a, X, bias, st) : launch_route_as<T, 32, false>(a, X, bias, st);
 }
 
