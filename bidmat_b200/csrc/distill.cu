@@ -320,7 +320,9 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
             mail_init_done();
             mail_expect(&arrived, l.parts * W * 8);
         }
-        cluster_arrive();               // every CTA has its barrier before anything is sent to it
+        // Every CTA has its barrier before anything is sent to it.  The warp that reads the student's logits of all entries, in
+        // every part of the column, arrives when it has read them: dX may be X, and no part is written before the sums are here.
+        if (part != 0 || tid < THREADS) cluster_arrive();
     }
     if (tid >= THREADS) {
         Held h;
@@ -354,7 +356,10 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
             slope = make_float2((float)e.P * w / a.t * qf, ref);
             if (e.P == 0.0) atomicOr(&twice, 2);
         }
-        if (MODE == BOTH) cluster_wait();
+        if (MODE == BOTH) {
+            if (part == 0) cluster_arrive();
+            cluster_wait();
+        }
         __syncthreads();                                        // marks, slope; the part is in shared memory
         if (MODE == BOTH) {
             const SumExp s = receive<W>(&arrived, joined, l.parts * W, a.c);
