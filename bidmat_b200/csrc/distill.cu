@@ -604,7 +604,8 @@ DistillArgs arguments(int nrows, long long ldx, long long lddx, float t, const T
 
 int check(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype, float temperature, const int *Zir,
           const int *Zjc, const float *Zdata) {
-    if (nrows < 1 || nrows > kMostRows || ncols < 0 || ncols > kMostRows || nnz < 0 || !dtype_ok(dtype)) return (int)cudaErrorInvalidValue;
+    if (nrows < 1 || nrows > kMostRows || ncols < 0 || ncols > kMostRows || nnz < 0 || nnz > kMostEntries || !dtype_ok(dtype))
+        return (int)cudaErrorInvalidValue;
     if (!temperature_ok(temperature)) return (int)cudaErrorInvalidValue;
     if (ncols == 0) return 0;
     if (!dense_ok(X, ldx, nrows, dtype) || !Zjc || (nnz > 0 && (!Zir || !Zdata))) return (int)cudaErrorInvalidValue;

@@ -800,7 +800,8 @@ extern "C" int bidmat_b200_route(int nrows, int ncols, const void *X, long long 
 extern "C" int bidmat_b200_route_grad(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype, int score,
                                       int renorm, float scale, const int *Sir, const int *Sjc, const float *Sdata,
                                       const float *dS, void *dX, long long lddx, bidmat_stream_t stream) {
-    if (!route_sizes_ok(nrows, ncols, score, scale) || !dtype_ok(dtype) || nnz < 0) return (int)cudaErrorInvalidValue;
+    if (!route_sizes_ok(nrows, ncols, score, scale) || !dtype_ok(dtype) || nnz < 0 || nnz > kMostEntries)
+        return (int)cudaErrorInvalidValue;
     if (ncols == 0) return 0;
     if (!dense_ok(X, ldx, nrows, dtype) || !dense_ok(dX, lddx, nrows, dtype) || !Sjc) return (int)cudaErrorInvalidValue;
     if (nnz > 0 && (!Sir || !Sdata || !dS)) return (int)cudaErrorInvalidValue;

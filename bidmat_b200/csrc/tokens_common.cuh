@@ -54,8 +54,8 @@ __device__ __forceinline__ double warp_max(double v) {
 }
 
 // ------------------------------------------------------------------ host side
-// Rows and columns are counted in ints, with room for the steps of a loop.
-constexpr int kMostRows = 0x7fff0000;
+// Rows, columns and entries are counted in ints, with room for the steps of a loop.
+constexpr int kMostRows = 0x7fff0000, kMostEntries = 0x7fff0000;
 
 inline size_t dtype_size(int dtype) { return dtype == BIDMAT_B200_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == BIDMAT_B200_F32 || dtype == BIDMAT_B200_BF16 || dtype == BIDMAT_B200_F16; }

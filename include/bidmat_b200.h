@@ -420,7 +420,8 @@ BIDMAT_B200_API int bidmat_b200_route(int nrows, int ncols, const void *X, long 
  * order of Sdata), with S as bidmat_b200_route left it for the same score, renorm and scale.  All of dX is
  * written: rows that no entry names get 0, or, for a softmax without renorm, their share of the
  * normalisation.  The choice itself and the bias have no gradient.  Columns may hold any number of entries;
- * entries whose row is outside the matrix are left out.  dX may be X (with the same ld). */
+ * entries whose row is outside the matrix are left out.  nnz is at most 2^31 - 65536.  dX may be X (with
+ * the same ld). */
 BIDMAT_B200_API int bidmat_b200_route_grad(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
                                            int score, int renorm, float scale, const int *Sir, const int *Sjc,
                                            const float *Sdata, const float *dS, void *dX, long long lddx,
@@ -454,7 +455,7 @@ BIDMAT_B200_API int bidmat_b200_top_logits(int nrows, int ncols, const void *X, 
  * whose row is outside the matrix makes its column's results NaN; a row that comes twice counts with the
  * sum of its p.  A NaN or +infinity among a column's logits, or a column of -infinity, makes its results
  * NaN (in fp32, so also in fp16 outputs; finite gradients above 65504 become infinite there).
- * dX may be X (with the same ld). */
+ * nnz is at most 2^31 - 65536.  dX may be X (with the same ld). */
 BIDMAT_B200_API int bidmat_b200_distill(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
                                         float temperature, const int *Zir, const int *Zjc, const float *Zdata,
                                         const float *Zlse, float *loss, float *Xlse, bidmat_stream_t stream);
