@@ -387,7 +387,8 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
     }
 
     x.template arrive<THREADS>(kept, X, end, X + col * a.ldx, a.nrows);
-    float f, ref, f_exact = 0.f;    // f_exact: relative to the reference itself
+    float f, ref;
+    SumExp sum;                     // of the column
     if (MODE == BOTH) {
         SumExp s;
 #pragma unroll 4
@@ -415,10 +416,9 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
         cluster_wait();
         if (lane < l.parts) mail_send(&joined[part * W + (tid >> 5)], &arrived, lane, make_float2(s.m, s.s));
         __syncthreads();
-        const SumExp sum = receive<W>(&arrived, joined, l.parts * W, a.c);
+        sum = receive<W>(&arrived, joined, l.parts * W, a.c);
         ref = sum.ref();
         f = slope.x / sum.s;
-        f_exact = slope.x / (float)sum.exact(a.c);
     } else {
         __syncthreads();
         f = slope.x;
@@ -457,8 +457,9 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
             store(i, Pack<T>::pack(v));
         }
     } else {
-        // differences first: references beyond 1e37, negative weights in 16 bits, fp32 gradients from a saved log-sum-exp
-        const float f1 = MODE == BOTH && moderate(k0) ? f_exact : f;
+        // differences first: references that are not moderate, negative weights in 16 bits, fp32 gradients from a saved
+        // log-sum-exp.  They are relative to the reference itself, and so is the sum.
+        const float f1 = MODE == BOTH ? slope.x / (float)sum.exact(a.c) : f;
         const unsigned long long mr = pair(-ref, -ref), cc = pair(a.c, a.c), ff = pair(f1, f1);
 #pragma unroll 2
         for (int i = tid; i < x.n; i += THREADS) {

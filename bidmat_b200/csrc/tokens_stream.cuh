@@ -7,9 +7,10 @@
 // well (between its first element and its last), and written one element at a time.
 //
 // A thread keeps (m, s): the largest x so far and the sum of 2^(x c - k) over its rows, c = log2(e)/t and k = m c as fp32
-// rounds it.  That takes one instruction for two differences, and k's rounding is made up for where the sum is used
-// (exact()).  Where m c is beyond 1e37 (a mask of the type's lowest value that leaves nothing, say) the differences
-// x - m come first instead, so that such a column neither overflows nor loses its uniform distribution.
+// rounds it.  That takes one instruction for two differences.  The terms are then relative to 2^k and not to 2^(m c), which
+// exact() makes up for by the factor 2^(k - m c), the exponent taken in fp64, where m c has no rounding.  Up to |k| = 2^24 it
+// is at most a half.  Beyond that (a mask of -1e9 that leaves nothing, logits over a temperature of 1e-7) the differences
+// x - m come first instead, so that such a column neither overflows nor loses its distribution.
 #pragma once
 #include <cooperative_groups.h>
 
@@ -18,7 +19,6 @@
 namespace bidmat {
 
 constexpr double kLog2e = 1.4426950408889634074;
-constexpr double kLn2 = 0.69314718055994530942;
 
 __device__ __forceinline__ float exp2_fast(float x) {
     float y;
@@ -216,11 +216,13 @@ __device__ __forceinline__ bool mail_wait(unsigned long long *bar, unsigned pari
 }
 
 // k of a maximum, and whether exponents are taken relative to it.
-__device__ __forceinline__ bool moderate(float k) { return fabsf(k) <= 1e37f; }
-// The exponent that brings a sum relative to m1 up to m2 >= m1.
+__device__ __forceinline__ bool moderate(float k) { return fabsf(k) <= 16777216.f; }
+// The exponent that brings a sum relative to m1 up to m2 >= m1.  Where only one of them is moderate the other's sum is
+// relative to the maximum itself.
 __device__ __forceinline__ float rise(float m1, float m2, float c) {
     const float k1 = __fmul_rn(m1, c), k2 = __fmul_rn(m2, c);
-    return moderate(k1) && moderate(k2) ? k1 - k2 : (m1 - m2) * c;
+    if (moderate(k1) && moderate(k2)) return k1 - k2;
+    return (m1 - m2) * c - (moderate(k1) ? fmaf(m1, c, -k1) : 0.f) + (moderate(k2) ? fmaf(m2, c, -k2) : 0.f);
 }
 
 struct SumExp {
@@ -234,7 +236,7 @@ struct SumExp {
     // the sum of exp((x - m)/t)
     __device__ __forceinline__ double exact(float c) const {
         const float k = __fmul_rn(ref(), c);
-        return moderate(k) ? s * (1.0 - ((double)ref() * c - k) * kLn2) : (double)s;
+        return moderate(k) ? s * exp2(k - (double)ref() * c) : (double)s;
     }
     // log sum exp(x/t)
     __device__ __forceinline__ double log_sum(float t, float c) const {

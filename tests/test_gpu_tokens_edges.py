@@ -75,3 +75,109 @@ def test_distill_in_place_with_entries_in_every_part(cuda_device, dtype, V, T, k
         y = matrix(x.clone())
         again, _ = tokens.distillWithGrad(y, Z, temperature=2.0, omat=y)
         assert torch.equal(again.t, loss.t) and torch.equal(y.t, dX.t)
+
+
+# ------------------------------------------------------------------------------------------ large maxima
+#
+# Exponents are those of the differences from the largest logit, however large it is against the temperature.  The
+# definition is taken from the differences too: next to 1e20 the ordinary one loses its logarithms in 64 bits as well.
+# With d = (max - x)/t, of which what is beyond 104 leaves the range of fp32:
+#   sum of exponentials, relative   e = u (2 max d + V/256 + 16): an argument is off by at most 2 u d (its own rounding and that
+#                                   of log2(e)/t), ex2 by 4 u, a thread adds V/512 terms or fewer, the rest is for joining them
+#   log-sum-exp                     e + u |L|
+#   loss                            e + 4 u (1 + |loss|)
+#   gradient                        |w|/t (q (e + u (2 d + 8)) + 4 u p) + h |gradient|, and half the smallest number
+# and from a saved log-sum-exp S, where q = exp(x/t - S) may be far from a distribution, with d = |x/t - S| + u |S|:
+#   gradient                        |w|/t (q (u (2 d + 12) + 2^-50 |S|) + 4 u p) + h |gradient|
+SMALLEST = {"fp32": 2.0 ** -126, "bf16": 2.0 ** -126, "fp16": 2.0 ** -25}
+
+
+def close(got, want, tol, what):
+    got, want, tol = (np.asarray(v, np.float64) for v in (got, want, tol))
+    bad = ~(np.abs(got - want) <= tol)
+    if bad.any():
+        i = tuple(int(v[0]) for v in np.nonzero(bad))
+        raise AssertionError("%s: %d of %d outside, first at %s: got %r want %r tolerance %r"
+                             % (what, bad.sum(), bad.size, i, got[i], want[i], np.broadcast_to(tol, got.shape)[i]))
+
+
+def by_differences(x, t):
+    """(d, q, log of the sum of exp(-d)) of the rows of x"""
+    d = (x.max(1, keepdims=True) - x) / t
+    e = np.exp(-d)
+    s = e.sum(1, keepdims=True)
+    return d, e / s, np.log(s[:, 0])
+
+
+def large_columns(dtype, t, V, rng):
+    if t < 0.1:
+        at = [14.0, -60.0, 300.0, -3000.0]
+    else:
+        at = [300.0, -3e3, 3e4, -6e4]
+        if dtype != "fp16":
+            at += [-1e5, 1e6, -1e7, 1e8, -1e8, -1e9, 1e10, -1e20, 1e30, -1e37, 2e38]
+    at = [a for a in at for _ in range(2)]
+    x = np.array(at)[:, None] + np.where(np.arange(len(at)) % 2, 3.0 * t, 0.0)[:, None] * rng.standard_normal((len(at), V))
+    return torch.as_tensor(x, device="cuda").to(DT[dtype])
+
+
+@pytest.mark.parametrize("V", [300, 9001, 60000, 300007])
+@pytest.mark.parametrize("t", [1.0, 2.5, 1e-4, 1e-7])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_log_sum_exp_of_large_maxima(cuda_device, dtype, t, V):
+    x = large_columns(dtype, t, V, np.random.default_rng(V))
+    T, t32 = x.shape[0], float(np.float32(t))
+    xs = x.double().cpu().numpy()
+    d, _, logs = by_differences(xs, t32)
+    L = xs.max(1) / t32 + logs
+    tol = U * (2 * np.minimum(d, 104).max(1) + V / 256 + 16) + U * np.abs(L)
+    lse = row(np.zeros(T), cuda_device)
+    tokens.topLogits(matrix(x), 5, temperature=t, lse=lse)
+    close(lse.t.cpu().numpy()[:, 0], L, tol, "log-sum-exp of topLogits")
+    Z = sparse(V, T, np.arange(T + 1), np.zeros(T), np.zeros(T), cuda_device)
+    _, out = tokens.distill(matrix(x), Z, temperature=t)
+    close(out.t.cpu().numpy()[:, 0], L, tol, "log-sum-exp of distill")
+
+
+def check_large_gradients(device, dtype, t, V):
+    rng = np.random.default_rng(V + 1)
+    x = large_columns(dtype, t, V, rng)
+    T, t32 = x.shape[0], float(np.float32(t))
+    xs = x.double().cpu().numpy()
+    k = min(V, 200)
+    ir = np.stack([rng.permutation(V)[:k] for _ in range(T)])
+    z = np.float32(t * rng.standard_normal((T, k)))
+    w = np.full(T, np.float32(t * (1024 if dtype == "fp16" else 1)))
+    Z = sparse(V, T, np.arange(T + 1) * k, ir.ravel(), z.ravel(), device)
+    d, q, logs = by_differences(xs, t32)
+    _, pz, logz = by_differences(z.astype(np.float64), t32)
+    p = np.zeros((T, V))
+    np.put_along_axis(p, ir, pz, 1)
+    wt = w.astype(np.float64)[:, None] / t32
+    e = U * (2 * np.minimum(d, 104).max(1) + V / 256 + 16)
+    zd, xd = (z.max(1, keepdims=True).astype(np.float64) - z) / t32, np.take_along_axis(d, ir, 1)
+    loss = (pz * (xd - zd)).sum(1) + logs - logz
+    want = wt * (q - p)
+    got, dX = tokens.distillWithGrad(matrix(x), Z, weights=row(w, device), temperature=t)
+    close(dX.t.double().cpu().numpy(), want, wt * (q * (e[:, None] + U * (2 * np.minimum(d, 104) + 8)) + 4 * U * p)
+          + HALF[dtype] * np.abs(want) + SMALLEST[dtype] * (1 + wt), "gradient")
+    out, L = tokens.distill(matrix(x), Z, temperature=t)
+    S = L.t.double().cpu().numpy()
+    some = (np.abs(S[:, 0]) <= 2e8) & np.isfinite(S[:, 0])
+    S = S[some]
+    q = np.exp(xs[some] / t32 - S)
+    far = np.minimum(np.abs(xs[some] / t32 - S) + U * np.abs(S), 104)
+    want = wt[some] * (q - p[some])
+    dX = tokens.distillGrad(matrix(x), Z, L, weights=row(w, device), temperature=t)
+    close(dX.t.double().cpu().numpy()[some], want, wt[some] * (q * (U * (2 * far + 12) + 2.0 ** -50 * np.abs(S)) + 4 * U * p[some])
+          + HALF[dtype] * np.abs(want) + SMALLEST[dtype] * (1 + wt[some]), "gradient from the saved log-sum-exp")
+    return loss, e, out.t.cpu().numpy()[:, 0], w, got.t.cpu().numpy()[:, 0], np.abs(xs).max(1) / t32
+
+
+@pytest.mark.parametrize("V", [300, 9001, 60000, 300007])
+@pytest.mark.parametrize("t", [1.0, 2.5, 1e-4, 1e-7])
+def test_gradients_of_large_maxima(cuda_device, t, V):
+    loss, e, out, w, weighted, at = check_large_gradients(cuda_device, "fp32", t, V)
+    tol, some = e + 4 * U * (1 + np.abs(loss)), at < 1e6
+    close(out[some], loss[some], tol[some], "loss")
+    close(weighted[some], (w * loss)[some], (w * tol)[some], "weighted loss")
