@@ -435,13 +435,16 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
                 if (!((skip >> j) & 1u)) out[(long long)i * N + j] = reinterpret_cast<const T *>(&y)[j];
         }
     };
-    // exponents relative to the reference, for 16-bit gradients with the factor among them (its logarithm costs them nothing
-    // they could tell: 2^-24 of an exponent of 30 or so)
+    // Exponents relative to the reference, for 16-bit gradients with the factor among them.  Its logarithm makes for a second
+    // rounding that no sum makes up for, so the reference has to be small for that: with |k0| <= 256 and a factor within fp32's
+    // range it is at most half a step below 512, 2^-16 of an exponent, and that of k0 in GRAD 2^-17, together 1.6e-5 of the value
+    // (half a step of fp16 is 4.9e-4).
     constexpr bool FOLD = sizeof(T) == 2;
     const float k0 = __fmul_rn(ref, a.c), shift = FOLD ? k0 - log2f(fabsf(f)) : k0;
+    const bool quick = FOLD ? fabsf(k0) <= 256.f && !(f < 0.f) : MODE == BOTH && moderate(k0);
     if (zero) {
         for (int i = tid; i < x.n; i += THREADS) store(i, make_uint4(0, 0, 0, 0));
-    } else if (moderate(k0) && !(MODE == GRAD && !FOLD) && !(FOLD && f < 0.f)) {
+    } else if (quick) {
         const unsigned long long cc = pair(a.c, a.c), mk = pair(-shift, -shift), ff = pair(f, f);
 #pragma unroll 2
         for (int i = tid; i < x.n; i += THREADS) {
@@ -457,8 +460,8 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
             store(i, Pack<T>::pack(v));
         }
     } else {
-        // differences first: references that are not moderate, negative weights in 16 bits, fp32 gradients from a saved
-        // log-sum-exp.  They are relative to the reference itself, and so is the sum.
+        // differences first: references that are not moderate, or not small, or negative weights in 16 bits, fp32 gradients
+        // from a saved log-sum-exp.  They are relative to the reference itself, and so is the sum.
         const float f1 = MODE == BOTH ? slope.x / (float)sum.exact(a.c) : f;
         const unsigned long long mr = pair(-ref, -ref), cc = pair(a.c, a.c), ff = pair(f1, f1);
 #pragma unroll 2

@@ -89,6 +89,9 @@ def test_distill_in_place_with_entries_in_every_part(cuda_device, dtype, V, T, k
 #   gradient                        |w|/t (q (e + u (2 d + 8)) + 4 u p) + h |gradient|, and half the smallest number
 # and from a saved log-sum-exp S, where q = exp(x/t - S) may be far from a distribution, with d = |x/t - S| + u |S|:
 #   gradient                        |w|/t (q (u (2 d + 12) + 2^-50 |S|) + 4 u p) + h |gradient|
+# 16-bit gradients may have their factor in the exponent, two roundings of at most 2^-16 and 2^-17 there: (2^-16 + 2^-17) log 2
+# of q besides.
+FACTOR = {"fp32": 0.0, "bf16": (2.0 ** -16 + 2.0 ** -17) * np.log(2), "fp16": (2.0 ** -16 + 2.0 ** -17) * np.log(2)}
 SMALLEST = {"fp32": 2.0 ** -126, "bf16": 2.0 ** -126, "fp16": 2.0 ** -25}
 
 
@@ -159,7 +162,7 @@ def check_large_gradients(device, dtype, t, V):
     loss = (pz * (xd - zd)).sum(1) + logs - logz
     want = wt * (q - p)
     got, dX = tokens.distillWithGrad(matrix(x), Z, weights=row(w, device), temperature=t)
-    close(dX.t.double().cpu().numpy(), want, wt * (q * (e[:, None] + U * (2 * np.minimum(d, 104) + 8)) + 4 * U * p)
+    close(dX.t.double().cpu().numpy(), want, wt * (q * (e[:, None] + U * (2 * np.minimum(d, 104) + 8) + FACTOR[dtype]) + 4 * U * p)
           + HALF[dtype] * np.abs(want) + SMALLEST[dtype] * (1 + wt), "gradient")
     out, L = tokens.distill(matrix(x), Z, temperature=t)
     S = L.t.double().cpu().numpy()
@@ -169,7 +172,7 @@ def check_large_gradients(device, dtype, t, V):
     far = np.minimum(np.abs(xs[some] / t32 - S) + U * np.abs(S), 104)
     want = wt[some] * (q - p[some])
     dX = tokens.distillGrad(matrix(x), Z, L, weights=row(w, device), temperature=t)
-    close(dX.t.double().cpu().numpy()[some], want, wt[some] * (q * (U * (2 * far + 12) + 2.0 ** -50 * np.abs(S)) + 4 * U * p[some])
+    close(dX.t.double().cpu().numpy()[some], want, wt[some] * (q * (U * (2 * far + 12) + 2.0 ** -50 * np.abs(S) + FACTOR[dtype]) + 4 * U * p[some])
           + HALF[dtype] * np.abs(want) + SMALLEST[dtype] * (1 + wt[some]), "gradient from the saved log-sum-exp")
     return loss, e, out.t.cpu().numpy()[:, 0], w, got.t.cpu().numpy()[:, 0], np.abs(xs).max(1) / t32
 
@@ -181,3 +184,10 @@ def test_gradients_of_large_maxima(cuda_device, t, V):
     tol, some = e + 4 * U * (1 + np.abs(loss)), at < 1e6
     close(out[some], loss[some], tol[some], "loss")
     close(weighted[some], (w * loss)[some], (w * tol)[some], "weighted loss")
+
+
+@pytest.mark.parametrize("V", [300, 9001, 60000, 300007])
+@pytest.mark.parametrize("t", [1.0, 2.5, 1e-4, 1e-7])
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_gradients_of_large_maxima_in_16_bits(cuda_device, dtype, t, V):
+    check_large_gradients(cuda_device, dtype, t, V)
