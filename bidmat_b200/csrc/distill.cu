@@ -5,8 +5,9 @@
 //   L = log sum_v exp(x_v/t)
 //   loss = sum_i p_i (log p_i - (x_i/t - L)) = sum_i p_i (z_i - x_i)/t + P (L - Lt)
 //   d(w loss)/dx_v = w/t (P exp(x_v/t - L) - p_v)
-// The second form of the loss keeps the difference z - x, so it stays exact where the two agree.  What is
-// computed once per entry or once per column is in fp64; exponentials over the rows and their sums are in fp32.
+// The second form of the loss keeps the difference z - x, so it stays exact where the two agree; z is taken relative to the
+// entries' largest, x to the largest logit at an entry, so that neither loses anything where all are masked by a large number.
+// Masses and the loss are in fp64; exponentials over the rows, their sums and the gradient are in fp32.
 //
 // All three functions are bound by memory: one read of X, for the gradient one write of dX.
 #include <cuda_runtime.h>
@@ -29,8 +30,10 @@ struct Teacher {
 
 // What a column's entries amount to.
 struct Entries {
-    double lt, P;      // log-sum-exp and mass; P = 0: nothing to learn from, P = NaN: a row outside the matrix
-    double cross;      // sum p (z - x)/t
+    double zr, lt;     // p = exp((z - zr)/t - lt): the largest z and the log-sum-exp relative to it, or 0 and the one given
+    double P;          // mass; 0: nothing to learn from, NaN: a row outside the matrix
+    double xr;         // a logit next to the largest at an entry
+    double cross;      // sum p ((z - zr) - (x - xr))/t
 };
 
 // Entries that a warp has in registers: the first 32 R of a column.
@@ -53,13 +56,13 @@ __device__ __forceinline__ void hold(Held &h, const Teacher &z, int j0, int j1) 
 }
 
 // By one warp.  x: the student's column, read WITH_X.  xr, pr: the student's logits and the masses of the
-// entries held.  One exponential each.
+// entries held.  it: 1/t; differences times it are as near as differences over t.  One exponential each.
 template <typename T, bool WITH_X>
-__device__ __forceinline__ Entries weigh_entries(const Held &h, const Teacher &z, long long c, int nrows, double t, const T *x,
+__device__ __forceinline__ Entries weigh_entries(const Held &h, const Teacher &z, long long c, int nrows, double it, const T *x,
                                                  float (&xr)[R], float (&pr)[R]) {
     const int lane = threadIdx.x & 31;
-    double shift = 0.0;
-    if (z.lse) shift = z.lse[c];
+    double lt = 0.0, zr = 0.0, near = 0.0;
+    if (z.lse) lt = z.lse[c];
     bool outside = false;
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -74,13 +77,21 @@ __device__ __forceinline__ Entries weigh_entries(const Held &h, const Teacher &z
         for (int r = 0; r < R; r++) m = max_nan(m, (double)h.z[r]);
         for (int j = rest; j < h.j1; j += 32) m = max_nan(m, (double)z.data[j]);
         m = warp_max(m);
-        shift = m == -INFINITY ? 0.0 : m / t;
+        zr = m == -INFINITY ? 0.0 : m;
+    }
+    if (WITH_X) {                       // the largest of those held is near enough
+        float top = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+            if (h.row[r] >= 0 && h.row[r] < nrows && fabsf(xr[r]) < INFINITY) top = fmaxf(top, xr[r]);
+        top = warp_top(top);
+        near = top == -INFINITY ? 0.f : top;
     }
     double s = 0.0, cross = 0.0;
     auto add = [&](float zj, float xj) {
-        const double e = exp(zj / t - shift);
+        const double e = exp((zj - zr) * it - lt);
         s += e;
-        if (WITH_X && e > 0.0) cross += e * (((double)zj - (double)xj) / t);
+        if (WITH_X && e > 0.0) cross += e * (((zj - zr) - (xj - near)) * it);
         return e;
     };
 #pragma unroll
@@ -98,12 +109,14 @@ __device__ __forceinline__ Entries weigh_entries(const Held &h, const Teacher &z
     if (WITH_X) cross = warp_sum(cross);
     outside = __any_sync(0xffffffffu, outside);
     Entries e;
+    e.zr = zr;
+    e.xr = near;
     if (z.lse) {
-        e.lt = shift;
+        e.lt = lt;
         e.P = s;
         e.cross = cross;
     } else {
-        e.lt = s == 0.0 ? INFINITY : shift + log(s);       // nothing finite: every p is zero
+        e.lt = s == 0.0 ? INFINITY : log(s);               // nothing finite: every p is zero
         e.P = s == 0.0 ? 0.0 : s / s;                       // one, or NaN
         e.cross = cross / s;
 #pragma unroll
@@ -117,7 +130,7 @@ __device__ __forceinline__ Entries weigh_entries(const Held &h, const Teacher &z
 // the teacher's.
 struct Slope {
     float t, c, w, ref, f;
-    double qf, lt, P;
+    double it, qf, zr, lt, P;
 };
 
 // One stretch of the gradient is the vectors [a0, a1) of a column, at most kMarkRows rows.  The rows with an
@@ -150,25 +163,24 @@ template <typename T>
 __device__ __forceinline__ void write_entries(const Column<T> &x, T *out, const Teacher &z, int j0, int j1, int a0, int a1,
                                               const Slope &g, bool twice, int who, int count) {
     constexpr int N = Pack<T>::N;
-    const double t = g.t;
     for (int j = j0 + who; j < j1; j += count) {
         const int row = z.ir[j];
         const long long u = (long long)row + x.shift - (long long)a0 * N;
         if (row < 0 || row >= x.rows || u < 0 || u >= (long long)(a1 - a0) * N) continue;
-        double p = exp(z.data[j] / t - g.lt);
+        double p = exp((z.data[j] - g.zr) * g.it - g.lt);
         if (twice) {                                    // a row's first entry adds them up in their order
             bool mine = true;
             p = 0.0;
             for (int i = j0; i < j1; i++)
                 if (z.ir[i] == row) {
                     mine &= i >= j;
-                    p += exp(z.data[i] / t - g.lt);
+                    p += exp((z.data[i] - g.zr) * g.it - g.lt);
                 }
             if (!mine) continue;
         }
         const float xv = to_float(x.base[u + (long long)a0 * N]);
-        const double q = exp(((double)xv - g.ref) / t) * g.qf;
-        out[u + (long long)a0 * N] = from_float<T>(g.P == 0.0 ? 0.f : (float)(g.w / t * (g.P * q - p)));
+        const double q = exp(((double)xv - g.ref) * g.it) * g.qf;
+        out[u + (long long)a0 * N] = from_float<T>(g.P == 0.0 ? 0.f : (float)(g.w * g.it * (g.P * q - p)));
     }
 }
 
@@ -256,6 +268,7 @@ struct DistillArgs {
     int nrows;
     long long ldx, lddx;
     float t, c;
+    double it;                      // 1/t
     Teacher z;
     const float *weights, *lse_in;
     float *loss, *lse_out;
@@ -281,10 +294,11 @@ template <int W> __device__ __forceinline__ SumExp receive(unsigned long long *a
     return s;
 }
 
+template <bool WITH_LSE>
 __device__ __forceinline__ void write_loss(const DistillArgs &a, long long col, const SumExp &s, const Entries &e, float w) {
-    const double L = s.log_sum(a.t, a.c);
-    if (a.lse_out) a.lse_out[col] = (float)L;
-    a.loss[col] = e.P == 0.0 ? 0.f : (float)((double)w * (e.cross + e.P * (L - e.lt)));
+    const double l = s.log_sum(a.c);
+    if (WITH_LSE) a.lse_out[col] = (float)(s.m * a.it + l);
+    a.loss[col] = e.P == 0.0 ? 0.f : (float)((double)w * (e.cross + e.P * ((s.m - e.xr) * a.it + l - e.lt)));
 }
 
 template <typename T, int THREADS, Mode MODE>
@@ -345,8 +359,8 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
         for (int r = 0; r < R; r++) mark_row(h.row[r]);
         for (int j = j0 + 32 * R + lane; j < j1; j += 32) mark_row(a.z.ir[j]);
         // only CTA 0 needs the student's logits of all entries, for the loss
-        Entries e = MODE == BOTH && part == 0 ? weigh_entries<T, true>(h, a.z, col, a.nrows, a.t, X + col * a.ldx, xr, pr)
-                                              : weigh_entries<T, false>(h, a.z, col, a.nrows, a.t, nullptr, xr, pr);
+        Entries e = MODE == BOTH && part == 0 ? weigh_entries<T, true>(h, a.z, col, a.nrows, a.it, X + col * a.ldx, xr, pr)
+                                              : weigh_entries<T, false>(h, a.z, col, a.nrows, a.it, nullptr, xr, pr);
         float ref = 0.f, qf = 1.f;
         if (MODE == GRAD) {
             ref = (float)((double)lse * a.t);
@@ -365,7 +379,7 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
             const SumExp s = receive<W>(&arrived, joined, l.parts * W, a.c);
             ref = s.ref();
             qf = (float)(1.0 / s.exact(a.c));
-            if (part == 0 && lane == 0) write_loss(a, col, s, e, w);
+            if (part == 0 && lane == 0) write_loss<false>(a, col, s, e, w);
         }
         const bool plain = (twice & 1) == 0;
         if (plain) {
@@ -379,7 +393,7 @@ distill_part_kernel(DistillArgs a, Layout l, const T *X, T *dX) {
             }
         }
         if (!plain || j1 - j0 > 32 * R) {
-            const Slope g{a.t, a.c, w, ref, 0.f, (double)qf, e.lt, e.P};
+            const Slope g{a.t, a.c, w, ref, 0.f, a.it, (double)qf, e.zr, e.lt, e.P};
             const Column<T> whole(X + col * a.ldx, a.nrows);
             write_entries<T>(whole, dX + col * a.lddx - x.shift, a.z, plain ? j0 + 32 * R : j0, j1, x.v0, x.v0 + x.n, g, !plain, lane, 32);
         }
@@ -513,7 +527,7 @@ distill_long_kernel(DistillArgs a, const T *X, T *dX) {
             Held h;
             float xr[R], pr[R];
             hold(h, a.z, j0, j1);
-            e = weigh_entries<T, true>(h, a.z, col, a.nrows, a.t, X + col * a.ldx, xr, pr);
+            e = weigh_entries<T, true>(h, a.z, col, a.nrows, a.it, X + col * a.ldx, xr, pr);
         }
         cluster_wait();
         if (rank == 0 && lane < (GRADIENT ? size : 1)) *cluster.map_shared_rank(&entries, lane) = e;
@@ -530,14 +544,14 @@ distill_long_kernel(DistillArgs a, const T *X, T *dX) {
     for (int i = lane; i < size * W; i += 32) join(s, joined[i].x, joined[i].y, a.c);
     warp_join(s, a.c);
     const Entries &e = entries;
-    if (rank == 0 && tid == 0) write_loss(a, col, s, e, w);
+    if (rank == 0 && tid == 0) write_loss<!GRADIENT>(a, col, s, e, w);
     if (GRADIENT) {
         if (e.P == 0.0) {
             write_zeros<T, kStream + 32>(x, out, v0, v1);
             return;
         }
         const double sum = s.exact(a.c);
-        const Slope g{a.t, a.c, w, s.ref(), (float)e.P * w / (a.t * (float)sum), 1.0 / sum, e.lt, e.P};
+        const Slope g{a.t, a.c, w, s.ref(), (float)e.P * w / (a.t * (float)sum), a.it, 1.0 / sum, e.zr, e.lt, e.P};
         write_gradient<T, kStream + 32>(x, out, a.z, j0, j1, v0, v1, g, marks, &twice);
     }
 }
@@ -603,7 +617,7 @@ template <typename T> cudaError_t launch_loss(const DistillArgs &a, int ncols, c
 
 DistillArgs arguments(int nrows, long long ldx, long long lddx, float t, const Teacher &z, const float *weights, const float *lse_in,
                       float *loss, float *lse_out) {
-    return DistillArgs{nrows, ldx, lddx, t, (float)(kLog2e / (double)t), z, weights, lse_in, loss, lse_out};
+    return DistillArgs{nrows, ldx, lddx, t, (float)(kLog2e / (double)t), 1.0 / (double)t, z, weights, lse_in, loss, lse_out};
 }
 
 int check(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype, float temperature, const int *Zir,

@@ -238,10 +238,10 @@ struct SumExp {
         const float k = __fmul_rn(ref(), c);
         return moderate(k) ? s * exp2(k - (double)ref() * c) : (double)s;
     }
-    // log sum exp(x/t)
-    __device__ __forceinline__ double log_sum(float t, float c) const {
+    // log sum exp((x - m)/t), or log sum exp(x/t) of a column of -infinity or NaN
+    __device__ __forceinline__ double log_sum(float c) const {
         if (m == -INFINITY) return s == 0.f ? -INFINITY : NAN;
-        return m / (double)t + log(exact(c));
+        return log(exact(c));
     }
 };
 

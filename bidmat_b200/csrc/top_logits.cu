@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int g
             join(s, v.x, v.y, a.c);
         }
         warp_join(s, a.c);
-        if (lane == 0) a.lse[col] = (float)s.log_sum(a.t, a.c);
+        if (lane == 0) a.lse[col] = (float)(s.m / (double)a.t + s.log_sum(a.c));
     }
     if (parts > 1) cluster.sync();                              // a part stays until it has been read
     if (part != 0) return;

@@ -191,3 +191,41 @@ def test_gradients_of_large_maxima(cuda_device, t, V):
 @pytest.mark.parametrize("dtype", ["bf16", "fp16"])
 def test_gradients_of_large_maxima_in_16_bits(cuda_device, dtype, t, V):
     check_large_gradients(cuda_device, dtype, t, V)
+
+
+@pytest.mark.parametrize("V", [300, 60000, 300007])
+@pytest.mark.parametrize("t", [1.0, 2.5])
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+def test_loss_of_large_logits(cuda_device, dtype, t, V):
+    """The student's logits, the teacher's or both next to a large number, masks that leave nothing among them."""
+    loss, e, out, w, weighted, _ = check_large_gradients(cuda_device, dtype, t, V)
+    tol = e + 4 * U * (1 + np.abs(loss))
+    close(out, loss, tol, "loss")
+    close(weighted, w * loss, w * tol, "weighted loss")
+    rng = np.random.default_rng(V + 2)
+    t32, k = float(np.float32(t)), min(V, 200)
+    low = torch.finfo(DT[dtype]).min
+    xs = [0.0, 0.0, 0.0, 0.0, low, low, -3e4, low]
+    zs = [-1e9, -1e20, torch.finfo(torch.float32).min, 1e7, torch.finfo(torch.float32).min, 0.0, -1e9, low]
+    T = len(xs)
+    x = torch.as_tensor(np.array(xs)[:, None] + rng.standard_normal((T, V)), device=cuda_device).to(DT[dtype])
+    x = torch.clamp(x, min=low)
+    z = np.float32(np.maximum(np.array(zs)[:, None] + rng.standard_normal((T, k)), float(np.finfo(np.float32).min)))
+    ir = np.stack([rng.permutation(V)[:k] for _ in range(T)])
+    Z = sparse(V, T, np.arange(T + 1) * k, ir.ravel(), z.ravel(), cuda_device)
+    x64 = x.double().cpu().numpy()
+    d, q, logs = by_differences(x64, t32)
+    zd, pz, logz = by_differences(z.astype(np.float64), t32)
+    loss = (pz * (np.take_along_axis(d, ir, 1) - zd)).sum(1) + logs - logz
+    e = U * (2 * np.minimum(d, 104).max(1) + V / 256 + 16)
+    out, L = tokens.distill(matrix(x), Z, temperature=t)
+    close(out.t.cpu().numpy()[:, 0], loss, e + 4 * U * (1 + np.abs(loss)), "loss of a large teacher")
+    w = np.full(T, np.float32(1024 * t))
+    got, dX = tokens.distillWithGrad(matrix(x), Z, weights=row(w, cuda_device), temperature=t)
+    close(got.t.cpu().numpy()[:, 0], w * loss, w * (e + 4 * U * (1 + np.abs(loss))), "weighted loss of a large teacher")
+    p = np.zeros((T, V))
+    np.put_along_axis(p, ir, pz, 1)
+    wt = 1024.0 * t / t32
+    want = wt * (q - p)
+    close(dX.t.double().cpu().numpy(), want, wt * (q * (e[:, None] + U * (2 * np.minimum(d, 104) + 8) + FACTOR[dtype]) + 4 * U * p)
+          + HALF[dtype] * np.abs(want) + SMALLEST[dtype] * (1 + wt), "gradient of a large teacher")
