@@ -36,6 +36,11 @@ struct Entries {
     double cross;      // sum p ((z - zr) - (x - xr))/t
 };
 
+// p of an entry, 0 for -infinity also where the log-sum-exp is -infinity (a teacher's column of nothing else).
+__device__ __forceinline__ double mass(float z, double zr, double it, double lt) {
+    return z == -INFINITY ? 0.0 : exp((z - zr) * it - lt);
+}
+
 // Entries that a warp has in registers: the first 32 R of a column.
 constexpr int R = 4;
 struct Held {
@@ -89,7 +94,7 @@ __device__ __forceinline__ Entries weigh_entries(const Held &h, const Teacher &z
     }
     double s = 0.0, cross = 0.0;
     auto add = [&](float zj, float xj) {
-        const double e = exp((zj - zr) * it - lt);
+        const double e = mass(zj, zr, it, lt);
         s += e;
         if (WITH_X && e > 0.0) cross += e * (((zj - zr) - (xj - near)) * it);
         return e;
@@ -167,14 +172,14 @@ __device__ __forceinline__ void write_entries(const Column<T> &x, T *out, const 
         const int row = z.ir[j];
         const long long u = (long long)row + x.shift - (long long)a0 * N;
         if (row < 0 || row >= x.rows || u < 0 || u >= (long long)(a1 - a0) * N) continue;
-        double p = exp((z.data[j] - g.zr) * g.it - g.lt);
+        double p = mass(z.data[j], g.zr, g.it, g.lt);
         if (twice) {                                    // a row's first entry adds them up in their order
             bool mine = true;
             p = 0.0;
             for (int i = j0; i < j1; i++)
                 if (z.ir[i] == row) {
                     mine &= i >= j;
-                    p += exp((z.data[i] - g.zr) * g.it - g.lt);
+                    p += mass(z.data[i], g.zr, g.it, g.lt);
                 }
             if (!mine) continue;
         }

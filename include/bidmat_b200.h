@@ -450,8 +450,9 @@ BIDMAT_B200_API int bidmat_b200_top_logits(int nrows, int ncols, const void *X, 
  *     saved Xlse: dX[v] = weights/t (P exp(X[v]/t - L) - p_v) with P = sum p_i.
  * distill_with_grad does both with one read of X; its loss is weights[c] loss[c] (the weights are known
  *     before the loss: a mean over tokens, a loss mask, a loss scale).
- * weights == NULL stands for ones.  Columns without an entry above -infinity have loss and gradient 0; so
- * have columns of weight 0 in the two functions that take weights, which do not read them.  An entry
+ * weights == NULL stands for ones.  Columns without an entry above -infinity have loss and gradient 0,
+ * whatever Zlse says (bidmat_b200_top_logits leaves -infinity there for such a teacher); so have
+ * columns of weight 0 in the two functions that take weights, which do not read them.  An entry
  * whose row is outside the matrix makes its column's results NaN; a row that comes twice counts with the
  * sum of its p.  A NaN or +infinity among a column's logits, or a column of -infinity, makes its results
  * NaN (in fp32, so also in fp16 outputs; finite gradients above 65504 become infinite there).

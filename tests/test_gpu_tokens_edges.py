@@ -229,3 +229,30 @@ def test_loss_of_large_logits(cuda_device, dtype, t, V):
     want = wt * (q - p)
     close(dX.t.double().cpu().numpy(), want, wt * (q * (e[:, None] + U * (2 * np.minimum(d, 104) + 8) + FACTOR[dtype]) + 4 * U * p)
           + HALF[dtype] * np.abs(want) + SMALLEST[dtype] * (1 + wt), "gradient of a large teacher")
+
+
+@pytest.mark.parametrize("dtype", ["fp32", "bf16"])
+@pytest.mark.parametrize("V,k", [(1000, 30), (70001, 200), (400003, 5)])
+def test_padded_tokens_of_a_teacher_are_nothing_to_learn_from(cuda_device, dtype, V, k):
+    """A teacher's columns of -infinity have the log-sum-exp -infinity; the loss and the gradient there are 0, also where the
+    student is masked as well, and the other columns are those of a batch without padding."""
+    g = torch.Generator(device=cuda_device)
+    g.manual_seed(V)
+    teach, stud = (torch.randn((6, V), generator=g, device=cuda_device).to(DT[dtype]) for _ in range(2))
+    teach[[1, 4, 5]] = -torch.inf
+    stud[4] = -torch.inf
+    lse = row(np.zeros(6), cuda_device)
+    Z = tokens.topLogits(matrix(teach), k, lse=lse)
+    assert torch.isneginf(lse.t[[1, 4, 5]]).all()
+    loss, L = tokens.distill(matrix(stud), Z, lse=lse)
+    wl, dX = tokens.distillWithGrad(matrix(stud), Z, lse=lse)
+    dY = tokens.distillGrad(matrix(stud), Z, L, lse=lse)
+    for out in (loss.t, wl.t, dX.t, dY.t):
+        assert bool((out[[1, 4, 5]] == 0).all()) and bool(torch.isfinite(out).all())
+    some = [0, 2, 3]
+    lse = row(np.zeros(3), cuda_device)
+    Z = tokens.topLogits(matrix(teach[some]), k, lse=lse)
+    # split over more or fewer CTAs a column may be summed up in another order: both are within e of the definition
+    e = 2 * U * (2 * float(stud[some].float().max() - stud[some].float().min()) + V / 256 + 16)
+    ones = tokens.distill(matrix(stud[some]), Z, lse=lse)[0]
+    assert bool((loss.t[some] - ones.t).abs().max() <= e + 8 * U * (1 + float(ones.t.abs().max())))
