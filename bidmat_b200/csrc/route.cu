@@ -474,6 +474,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     }
     int n = __shfl_sync(0xffffffffu, at, G - 1, G);
     at -= own;
+    bool left_out = false;                          // rows whose keys equal the bound in fp32 but are not all made of the same numbers
     if (__any_sync(0xffffffffu, n > L)) {
         // more than the list holds: those above the bound, and of those that equal it the lowest rows
         const bool over = n > L;
@@ -488,14 +489,19 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         const int first = n1 - own1;
         n1 = __shfl_sync(0xffffffffu, n1, G - 1, G);
         if (over && n1 + a.k > L) again = true;     // one lane has too many of the largest
-        int taken = n1;
+        int taken = n1, first_tie = -1;
         for (int e = sub; e - sub < a.nrows; e += G) {
             const bool tie = over && !again && e < a.nrows && val[e] == bound;
             const unsigned vote = (__ballot_sync(0xffffffffu, tie) & mine) >> (which * G);
             const int to = taken + __popc(vote & before_me);
             if (tie && to < L) list[to] = entry_of(bound, e);
             taken += __popc(vote);
+            if (BIAS && vote) {
+                if (first_tie < 0) first_tie = e - sub + __ffs(vote) - 1;
+                if (tie && (to_float(x[e]) != to_float(x[first_tie]) || bias[e] != bias[first_tie])) left_out = true;
+            }
         }
+        left_out = left_out && taken > L;
         if (over) {
             mask = again ? 0 : above;
             at = first;
@@ -539,19 +545,27 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     if (!none && n < a.k) again = true;             // fewer than k rows: the others are found there
     const Entry pick = sub < min(a.k, n) ? sorted[sub] : 0;
     if (BIAS) {
-        // neighbours among the picks, and the last one with what comes next
+        // Neighbours among the picks, and the last one with all that may come before it: behind rows that are made of the same
+        // numbers as the last pick there may be others.
 #pragma unroll
         for (int o = G / 2; o; o >>= 1) rejected = fmaxf(rejected, __shfl_xor_sync(0xffffffffu, rejected, o));
-        if (pick != 0) {
-            if (sub + 1 < n) {
-                const Entry q = sorted[sub + 1];
-                if (near(key_of(pick), key_of(q), within)) {
-                    const int r = row_of(pick), t = row_of(q);
-                    if (to_float(x[r]) != to_float(x[t]) || bias[r] != bias[t]) again = true;
-                }
-            } else if (rejected > -INFINITY && near(key_of(pick), rejected, within)) {
-                again = true;
+        auto same_numbers = [&](Entry p, Entry q) {
+            const int r = row_of(p), t = row_of(q);
+            return to_float(x[r]) == to_float(x[t]) && bias[r] == bias[t];
+        };
+        if (pick != 0 && sub + 1 < min(a.k, n)) {
+            const Entry q = sorted[sub + 1];
+            if (near(key_of(pick), key_of(q), within) && !same_numbers(pick, q)) again = true;
+        }
+        if (n >= a.k) {
+            const Entry last = sorted[a.k - 1];
+            for (int j = a.k + sub; j < n; j += G) {
+                const Entry q = sorted[j];
+                if (!near(key_of(last), key_of(q), within)) break;
+                if (!same_numbers(last, q)) again = true;
             }
+            if (rejected > -INFINITY && near(key_of(last), rejected, within)) again = true;
+            if (left_out && near(key_of(last), bound, within)) again = true;
         }
     }
     const unsigned redo_groups = __ballot_sync(0xffffffffu, groups_again && !bad && on);

@@ -9,6 +9,7 @@ import torch
 import tokens_oracle as oracle64
 from bidmat_b200 import tokens
 from bidmat_b200.mat import GHMat, GMat, GSMat
+from test_gpu_tokens import check_route
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -256,3 +257,35 @@ def test_padded_tokens_of_a_teacher_are_nothing_to_learn_from(cuda_device, dtype
     e = 2 * U * (2 * float(stud[some].float().max() - stud[some].float().min()) + V / 256 + 16)
     ones = tokens.distill(matrix(stud[some]), Z, lse=lse)[0]
     assert bool((loss.t[some] - ones.t).abs().max() <= e + 8 * U * (1 + float(ones.t.abs().max())))
+
+
+# ------------------------------------------------------------------------------------------ routing
+
+def up(v):
+    return np.nextafter(np.float32(v), np.float32(np.inf))
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,k", [(3, 1), (20, 5), (30, 8), (96, 1), (96, 12), (256, 8), (512, 16), (1024, 32)])
+def test_route_a_better_row_behind_identical_ones(cuda_device, score, E, k):
+    """Rows with the same score and bias around the k-th place, and behind them one that is better by less than fp32 can
+    tell after the bias has been added.  Weights and picks as in 64 bits."""
+    rng = np.random.default_rng(E + k)
+    places = sorted({E - 1, E // 2, k, 0} & set(range(E)))
+    x = np.ones((len(places) + 4, E), np.float32)
+    for i, p in enumerate(places):
+        x[i, p] = up(1.0)
+    x[-4] = 0.0
+    x[-3] = 0.5 * rng.integers(0, 2, E)
+    x[-2, : k // 2] = 3.0                                   # some picks far above, the rest among identical ones
+    x[-2, E - 1] = up(1.0)
+    x[-1] = np.where(rng.random(E) < 0.2, up(1.0), 1.0)
+    one = np.zeros(E)
+    one[E - 1] = 1e-9
+    steps = 0.25 + 2.0 ** -30 * rng.integers(0, 3, E)      # bias that moves in small fixed steps
+    for bias in (np.full(E, 0.25), one, steps, np.zeros(E)):
+        check_route(x, "fp32", cuda_device, k, score=score, bias=bias)
+        if E % 4 == 0 and k <= E // 2:
+            check_route(x, "fp32", cuda_device, k, score=score, bias=bias, groups=4, topgroups=2, renorm=False)
+    for bias in (one, steps):
+        check_route(np.round(2 * rng.standard_normal((300, E))) / 2, "bf16", cuda_device, k, score=score, bias=bias)
