@@ -243,8 +243,9 @@ __device__ __forceinline__ float key_of(Entry e) { return order_value((unsigned)
 // s = 1/(1 + e) is then off by at most s (1 - s) (2^-22 + |x| 2^-23) + 1.5 s 2^-23 < 2^-22 (the exponential, the sum and the
 // reciprocal), a softmax by at most 2^-20 of the column's largest (the sum's error besides).  Two sums of two of them that
 // differ by more than four times that, or sums with a bias that differ by more than twice that, and by more than
-// 2^-22 of their size for the roundings of the sums, are in the right order; so are keys made of the same two numbers.  A column
-// with two neighbours closer than that, one in some thousand, goes to route_few or route_exact.
+// 2^-22 of their size for the roundings of the sums, are in the right order; so are keys made of the same two numbers.  The size
+// of a group's sum is that of its two parts, which may have opposite signs with a bias.  A column with two neighbours closer than
+// that, one in some thousand, goes to route_few or route_exact.
 constexpr float kNearSigmoid = 9.5367432e-07f, kNearSoftmax = 3.8146973e-06f, kNearPart = 2.3841858e-07f;
 
 __device__ __forceinline__ bool near(float a, float b, float within) {
@@ -264,6 +265,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     char *const base = reinterpret_cast<char *>(route_smem) + (size_t)warp * a.warp_bytes;
     float *val = reinterpret_cast<float *>(base) + which * a.stride;
     float *gval = val + ((a.nrows + 3) & ~3);
+    float *goff = gval + a.ngroups;                 // BIAS: what the roundings of a group's sum may come to
     Entry *list = reinterpret_cast<Entry *>(base + a.lists_at) + which * 2 * L, *sorted = list + L;
     const bool on = c < a.ncols;
     const T *x = X + (on ? c : 0) * a.ldx;
@@ -366,10 +368,13 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
             } else {
                 for (int i = 0; i < size; i++) add(val[g * size + i]);
             }
-            gval[g] = a.grouptop == 2 && b2 > -INFINITY ? b1 + b2 : b1;
+            const bool both = a.grouptop == 2 && b2 > -INFINITY;
+            gval[g] = both ? fmaxf(b1 + b2, -3.4028235e38f) : b1;       // not that of a group of nothing
+            if (BIAS) goff[g] = kNearPart * fabsf(b1) + (both ? kNearPart * fabsf(b2) : 0.f);
         }
         __syncwarp();
-        float worst = INFINITY, best = -INFINITY;   // of the groups kept, of those dropped
+        // at least, at most: of the groups kept, of those dropped
+        float worst = INFINITY, best = -INFINITY;
         unsigned drop = 0;                          // of this lane's groups
         int n = 0;
         for (int g = sub; g < a.ngroups; g += G, n++) {
@@ -379,8 +384,9 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
                 const float u = gval[h];
                 before += u > v || (u == v && h < g);
             }
-            if (before < a.topgroups) worst = fminf(worst, v);
-            else best = fmaxf(best, v), drop |= 1u << (n & 31);
+            const float off = BIAS ? goff[g] : kNearPart * fabsf(v);
+            if (before < a.topgroups) worst = fminf(worst, v - off);
+            else best = fmaxf(best, v > -INFINITY ? v + off : v), drop |= 1u << (n & 31);
         }
         __syncwarp();
 #pragma unroll
@@ -388,7 +394,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
             worst = fminf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
             best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
         }
-        groups_again = (BIAS || group_scores) && best > -INFINITY && near(worst, best, within);
+        groups_again = (BIAS || group_scores) && best > -INFINITY && !(worst - best > within);
         n = 0;
         for (int g = sub; g < a.ngroups; g += G, n++) {
             if (!((drop >> (n & 31)) & 1u)) continue;
@@ -736,7 +742,7 @@ template <typename T, int G, bool BIAS>
 cudaError_t launch_route_as(RouteArgs a, const void *X, const float *bias, cudaStream_t st) {
     constexpr int C = 32 / G;
     const auto kernel = route_kernel<T, G, BIAS>;
-    a.stride = (((a.nrows + 3) / 4 * 4 + a.ngroups + 31) & ~31) + 8;              // columns 8 banks apart
+    a.stride = (((a.nrows + 3) / 4 * 4 + a.ngroups * (BIAS ? 2 : 1) + 31) & ~31) + 8;       // columns 8 banks apart
     a.wide = is16(X) && a.nrows % Pack<T>::N == 0 && (a.ldx % Pack<T>::N == 0 || a.ncols == 1);
     a.lists_at = C * a.stride * (int)sizeof(float);
     a.doubles_at = a.lists_at + C * 2 * kListed * G * (int)sizeof(Entry);

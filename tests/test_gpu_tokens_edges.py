@@ -289,3 +289,35 @@ def test_route_a_better_row_behind_identical_ones(cuda_device, score, E, k):
             check_route(x, "fp32", cuda_device, k, score=score, bias=bias, groups=4, topgroups=2, renorm=False)
     for bias in (one, steps):
         check_route(np.round(2 * rng.standard_normal((300, E))) / 2, "bf16", cuda_device, k, score=score, bias=bias)
+
+
+@pytest.mark.parametrize("E,groups,k", [(32, 8, 4), (64, 16, 8), (256, 8, 8), (512, 16, 16), (1024, 64, 32)])
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+def test_route_groups_whose_sums_cancel(cuda_device, score, E, groups, k):
+    """Biases that force rows on and off by +-1000, so that a group's sum is small against its parts and their roundings
+    in fp32 (1e-4 there) are larger than the differences between the groups; picks and weights as in 64 bits."""
+    rng = np.random.default_rng(E + groups)
+    x = 0.05 * rng.standard_normal((4000 if E <= 64 else 500, E))
+    size = E // groups
+    for on, off in ((1000.0, -1000.0), (37.5, -37.5), (1e6, -1e6)):
+        bias = np.full(E, -2e6)
+        bias[::size] = on
+        bias[1::size] = off
+        check_route(x, "fp32", cuda_device, min(k, size), score=score, bias=bias, groups=groups, topgroups=1 + groups // 2)
+        check_route(x, "bf16", cuda_device, 1, score=score, bias=bias + 0.001 * rng.standard_normal(E), groups=groups, topgroups=2)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups", [(256, 8), (1024, 16)])
+def test_route_groups_masked_by_the_lowest_bias(cuda_device, score, E, groups):
+    """Whole groups with the lowest number as their bias come behind all others and before groups of nothing but -infinity."""
+    rng = np.random.default_rng(E)
+    x = rng.standard_normal((50, E))
+    size = E // groups
+    x[10:, :size] = -np.inf                                 # group 0: nothing to pick from
+    x[20:, size:2 * size - 1] = -np.inf                     # group 1: one row is left
+    bias = 0.1 * rng.standard_normal(E)
+    bias[2 * size:4 * size] = np.finfo(np.float32).min      # groups 2 and 3: masked
+    for top in (1, 2, groups - 2, groups - 1, groups):
+        for grouptop in (1, 2):
+            check_route(x, "fp32", cuda_device, 3, score=score, bias=bias, groups=groups, topgroups=top, grouptop=grouptop)
