@@ -606,7 +606,8 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         const unsigned of = G == 32 ? 0xffffffffu : ((1u << G) - 1u) << (w2 * G);
         if (!(redo & of)) continue;
         const float last = __shfl_sync(0xffffffffu, pick != 0 ? key_of(pick) : -INFINITY, w2 * G + a.k - 1);
-        const float cut = last - 2.f * (__shfl_sync(0xffffffffu, within, w2 * G) + kNearPart * fabsf(last));
+        // no row that is out of the running, also where the last pick's key is the lowest number or so
+        const float cut = fmaxf(last - 2.f * (__shfl_sync(0xffffffffu, within, w2 * G) + kNearPart * fabsf(last)), -3.4028235e38f);
         const long long col = ((long long)blockIdx.x * kRouteWarps + warp) * C + w2;
         const T *xc = X + col * a.ldx;
         float *v = reinterpret_cast<float *>(base) + w2 * a.stride;

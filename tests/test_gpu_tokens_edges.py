@@ -321,3 +321,20 @@ def test_route_groups_masked_by_the_lowest_bias(cuda_device, score, E, groups):
     for top in (1, 2, groups - 2, groups - 1, groups):
         for grouptop in (1, 2):
             check_route(x, "fp32", cuda_device, 3, score=score, bias=bias, groups=groups, topgroups=top, grouptop=grouptop)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,groups,k", [(8, 2, 3), (24, 4, 3), (30, 5, 7), (32, 4, 8)])
+def test_route_few_rows_masked_by_the_lowest_bias(cuda_device, score, E, groups, k):
+    """Up to 32 rows of which fewer than k are unmasked: the masked ones follow by row, then those without a score."""
+    rng = np.random.default_rng(E)
+    x = rng.standard_normal((60, E))
+    x[20:40, ::3] = -np.inf
+    x[40:, : E // 2] = -np.inf
+    for open_rows in (1, 2, k - 1):
+        bias = np.full(E, np.finfo(np.float32).min)
+        bias[rng.permutation(E)[:open_rows]] = 0.25
+        for dtype in ("fp32", "bf16"):
+            check_route(x, dtype, cuda_device, k, score=score, bias=bias)
+            for top in range(1 + (k - 1) // (E // groups), groups + 1):
+                check_route(x, dtype, cuda_device, k, score=score, bias=bias, groups=groups, topgroups=top)
