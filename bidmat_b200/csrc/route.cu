@@ -701,7 +701,8 @@ route_grad_kernel(RouteArgs a, int nnz, const T *X, const int *__restrict__ Sir,
         for (int i = sub; i * 4 < a.nrows; i += G) *reinterpret_cast<float4 *>(col + i * 4) = make_float4(0.f, 0.f, 0.f, 0.f);
     }
     __syncwarp();
-    const float back = a.renorm ? d * (1.f / a.scale) : 0.f;
+    const float inverse = 1.f / a.scale;            // infinite for a subnormal scale
+    const float back = a.renorm ? (fabsf(inverse) < INFINITY ? d * inverse : d / a.scale) : 0.f;
     for (int j = j0; __any_sync(0xffffffffu, j < j1); j += G) {
         const bool have = j + sub < j1;
         const int row = have ? Sir[j + sub] : -1;

@@ -9,7 +9,7 @@ import torch
 import tokens_oracle as oracle64
 from bidmat_b200 import tokens
 from bidmat_b200.mat import GHMat, GMat, GSMat
-from test_gpu_tokens import check_route
+from test_gpu_tokens import check_route, grad_tolerance
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -338,3 +338,23 @@ def test_route_few_rows_masked_by_the_lowest_bias(cuda_device, score, E, groups,
             check_route(x, dtype, cuda_device, k, score=score, bias=bias)
             for top in range(1 + (k - 1) // (E // groups), groups + 1):
                 check_route(x, dtype, cuda_device, k, score=score, bias=bias, groups=groups, topgroups=top)
+
+
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("scale", [1e-39, -3e-39, 2.0 ** -127, 1e30, -0.5])
+@pytest.mark.parametrize("E", [40, 300])
+def test_route_gradient_of_tiny_and_large_scales(cuda_device, score, scale, E):
+    """Scales whose reciprocal is no number of fp32 among them; weights and their gradients make up for the scale, so that
+    the gradient of the scores is of ordinary size.  Tolerance as for other scales."""
+    rng = np.random.default_rng(E)
+    x = rng.standard_normal((20, E))
+    scale = float(np.float32(scale))
+    X = matrix(torch.as_tensor(x, device=cuda_device, dtype=torch.float32))
+    S = tokens.route(X, 6, score=score, scale=scale)
+    dS = S.copy()
+    dS.pdata = torch.as_tensor((rng.standard_normal(S.nnz) * min(abs(1.0 / scale), 1e38)).astype(np.float32), device=cuda_device)
+    got = tokens.routeGrad(X, S, dS, score=score, scale=scale).t.double().cpu().numpy()
+    xs, w, g = (v.double().cpu().numpy() for v in (X.t, S.pdata, dS.pdata))
+    want = oracle64.route_grad(xs, S.pjc.cpu().numpy(), S.pir.cpu().numpy(), w, g, score, True, scale)
+    assert np.abs(want).max() > 0.001          # a weight of 1e-39/6 and a gradient of 1e38 make 1/60, times 1 - s of a large sigmoid
+    close(got, want, grad_tolerance(xs, S, w, g, want, True, scale, "fp32"), "routeGrad at scale %g" % scale)
