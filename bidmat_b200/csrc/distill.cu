@@ -563,15 +563,20 @@ distill_long_kernel(DistillArgs a, const T *X, T *dX) {
 
 // ---------------------------------------------------------------- host side
 
+// Parts, 131072 x 2048 bf16.  BOTH: of 64 KB, three CTAs on an SM, 195 us; 32 KB and five CTAs 225 us, 48 KB and four 212 us,
+// 96 KB and two 221 us: with fewer parts fewer CTAs wait for one another.  GRAD: nobody waits, 32 KB and five CTAs.  A cluster has
+// at most 8 parts, so columns above 512 KB get parts of up to 96 KB and those above 768 KB are read twice.  Where columns
+// are few they are cut into more parts, to give every SM two CTAs.  Columns of up to 32 KB have CTAs of 96 threads
+// (8000 x 8192 bf16, BOTH: 83 us, 122 us with 288 threads).
+constexpr long long kGradBytes = 32768, kBothBytes = 65536, kMostPartBytes = 98304, kShortBytes = 32768;
+
 template <typename T, int THREADS, Mode MODE>
 cudaError_t launch_part(const DistillArgs &a, int ncols, int parts, long long nvec, const void *X, void *dX, cudaStream_t st) {
     const auto kernel = distill_part_kernel<T, THREADS, MODE>;
     const long long per = ((nvec + parts - 1) / parts + 7) & ~7LL;         // whole 128-byte lines
     const size_t smem = (size_t)per * 16 + (((size_t)per + 15) & ~size_t(15));
-    if (smem > 40000) {
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (err != cudaSuccess) return err;
-    }
+    const cudaError_t err = allow_shared(kernel, smem, (size_t)kMostPartBytes + kMostPartBytes / 16);
+    if (err != cudaSuccess) return err;
     if ((long long)ncols * parts > 0x7fffffffLL) return cudaErrorInvalidValue;
     cudaLaunchAttribute attr;
     const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)(ncols * parts), THREADS + 32, MODE == GRAD ? 1 : parts, smem, st);
@@ -586,13 +591,6 @@ cudaError_t launch_long(const DistillArgs &a, int ncols, int size, const void *X
     const cudaLaunchConfig_t cfg = cluster_config(&attr, (unsigned)(ncols * size), kStream + 32, size, 0, st);
     return cudaLaunchKernelEx(&cfg, distill_long_kernel<T, GRADIENT>, a, (const T *)X, (T *)dX);
 }
-
-// Parts, 131072 x 2048 bf16.  BOTH: of 64 KB, three CTAs on an SM, 195 us; 32 KB and five CTAs 225 us, 48 KB and four 212 us,
-// 96 KB and two 221 us: with fewer parts fewer CTAs wait for one another.  GRAD: nobody waits, 32 KB and five CTAs.  A cluster has
-// at most 8 parts, so columns above 512 KB get parts of up to 96 KB and those above 768 KB are read twice.  Where columns
-// are few they are cut into more parts, to give every SM two CTAs.  Columns of up to 32 KB have CTAs of 96 threads
-// (8000 x 8192 bf16, BOTH: 83 us, 122 us with 288 threads).
-constexpr long long kGradBytes = 32768, kBothBytes = 65536, kMostPartBytes = 98304, kShortBytes = 32768;
 
 template <typename T, Mode MODE>
 cudaError_t launch_distill(const DistillArgs &a, int ncols, const void *X, void *dX, cudaStream_t st) {

@@ -744,16 +744,19 @@ template <typename T, int G, bool BIAS>
 cudaError_t launch_route_as(RouteArgs a, const void *X, const float *bias, cudaStream_t st) {
     constexpr int C = 32 / G;
     const auto kernel = route_kernel<T, G, BIAS>;
-    a.stride = (((a.nrows + 3) / 4 * 4 + a.ngroups * (BIAS ? 2 : 1) + 31) & ~31) + 8;       // columns 8 banks apart
     a.wide = is16(X) && a.nrows % Pack<T>::N == 0 && (a.ldx % Pack<T>::N == 0 || a.ncols == 1);
-    a.lists_at = C * a.stride * (int)sizeof(float);
-    a.doubles_at = a.lists_at + C * 2 * kListed * G * (int)sizeof(Entry);
-    a.warp_bytes = (a.doubles_at + (a.nrows + a.ngroups) * (int)sizeof(double) + 15) & ~15;
-    const size_t smem = (size_t)kRouteWarps * a.warp_bytes;
-    if (smem > 40000) {
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-        if (err != cudaSuccess) return err;
-    }
+    auto place = [](RouteArgs &b) {
+        b.stride = (((b.nrows + 3) / 4 * 4 + b.ngroups * (BIAS ? 2 : 1) + 31) & ~31) + 8;       // columns 8 banks apart
+        b.lists_at = C * b.stride * (int)sizeof(float);
+        b.doubles_at = b.lists_at + C * 2 * kListed * G * (int)sizeof(Entry);
+        b.warp_bytes = (b.doubles_at + (b.nrows + b.ngroups) * (int)sizeof(double) + 15) & ~15;
+        return (size_t)kRouteWarps * b.warp_bytes;
+    };
+    RouteArgs most = a;
+    most.nrows = most.ngroups = 32 * G;             // launch_route
+    const size_t smem = place(a);
+    const cudaError_t err = allow_shared(kernel, smem, place(most));
+    if (err != cudaSuccess) return err;
     const long long per = (long long)kRouteWarps * C;
     kernel<<<(unsigned)((a.ncols + per - 1) / per), kRouteWarps * 32, smem, st>>>(a, (const T *)X, bias);
     return cudaGetLastError();

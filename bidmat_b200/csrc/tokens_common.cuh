@@ -68,6 +68,13 @@ inline bool dense_ok(const void *p, long long ld, int nrows, int dtype) {
     return p && ld >= nrows && (reinterpret_cast<uintptr_t>(p) & (dtype_size(dtype) - 1)) == 0;
 }
 
+// Dynamic shared memory above the 48 KB that every kernel may have: the kernel is allowed the most that any call asks for, not
+// what this one does, so that calls from two host threads do not take it away from one another.
+template <typename K> inline cudaError_t allow_shared(K kernel, size_t bytes, size_t most) {
+    if (bytes <= 40000) return cudaSuccess;
+    return cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
+}
+
 #define DISPATCH_DTYPE(DT, CALL)                                   \
     do {                                                           \
         if ((DT) == BIDMAT_B200_F32) { CALL(float); }              \

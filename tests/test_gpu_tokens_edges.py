@@ -2,6 +2,9 @@
 
 Against definitions in 64 bits (tokens_oracle), with the tolerances named at each test, where u = 2^-24 is half a
 step of fp32 and h half a step of the output type (2^-24 fp32, 2^-8 bf16, 2^-11 fp16)."""
+import sys
+import threading
+
 import numpy as np
 import pytest
 import torch
@@ -358,3 +361,59 @@ def test_route_gradient_of_tiny_and_large_scales(cuda_device, score, scale, E):
     want = oracle64.route_grad(xs, S.pjc.cpu().numpy(), S.pir.cpu().numpy(), w, g, score, True, scale)
     assert np.abs(want).max() > 0.001          # a weight of 1e-39/6 and a gradient of 1e38 make 1/60, times 1 - s of a large sigmoid
     close(got, want, grad_tolerance(xs, S, w, g, want, True, scale, "fp32"), "routeGrad at scale %g" % scale)
+
+
+# ------------------------------------------------------------------------------------------ several at once
+
+def test_calls_of_different_sizes_from_two_host_threads(cuda_device):
+    """The same kernels with different amounts of shared memory, called from two threads at once: every call is launched and
+    gives what it gives alone."""
+    from bidmat_b200 import _lib
+
+    def scores(E):
+        return matrix(torch.randn((8, E), device=cuda_device))
+
+    def arguments(X, S, stream):
+        return (X.nrows, X.ncols, X.pdata, X.nrows, 0, 32, 0, 0, 1, 1, 2, 1, 1.0, S.pir.data_ptr(), S.pic.data_ptr(),
+                S.pjc.data_ptr(), S.pdata.data_ptr(), stream.cuda_stream)
+
+    jobs = []
+    for E, V in ((1024, 32768), (700, 20000)):
+        x = matrix(torch.randn((300, V), device=cuda_device).to(torch.bfloat16))
+        r, Z = scores(E), tokens.topLogits(x, 4)
+        jobs.append((r, tokens.route(r, 32), x, Z, tokens.distillWithGrad(x, Z)))
+    torch.cuda.synchronize()
+    failed, start = [], threading.Barrier(2, timeout=60)
+
+    def run(r, S, x, Z, want):
+        try:
+            torch.cuda.set_device(cuda_device)
+            stream, T, out = torch.cuda.Stream(), S.copy(), matrix(torch.empty_like(x.t))
+            args = arguments(r, T, stream)
+            torch.cuda.synchronize()
+            start.wait()
+            for i in range(30000):
+                err = _lib.lib.bidmat_b200_route(*args)
+                assert err == 0, _lib.error_string(err)
+                if i % 500 == 0:
+                    stream.synchronize()
+            with torch.cuda.stream(stream):
+                for i in range(300):
+                    loss, _ = tokens.distillWithGrad(x, Z, omat=out)
+            stream.synchronize()
+            assert torch.equal(T.pir, S.pir) and torch.equal(T.pdata, S.pdata)
+            assert torch.equal(loss.t, want[0].t) and torch.equal(out.t, want[1].t)
+        except Exception as e:                              # the thread's, for the test to raise
+            failed.append(e)
+
+    before = sys.getswitchinterval()
+    sys.setswitchinterval(1e-5)
+    try:
+        threads = [threading.Thread(target=run, args=job) for job in jobs]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+    finally:
+        sys.setswitchinterval(before)
+    assert not failed, failed
