@@ -415,7 +415,10 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     const int before_me = (1 << sub) - 1;
     // ... of two maxima per lane, or of one where that is plenty: the bound stays well inside them, so that few more reach it
     const bool two = G < 32 || a.k > 12;
-    if (BIAS || a.ngroups > 1) {                    // other keys than the scores, or not all of them
+    // Other keys than the scores, or not all of them, or so few vectors that k + 1 of their maxima, of whole vectors each, are no
+    // bound to speak of: then the lists overflow and every column goes to route_exact.  (32768 columns, bf16, this and the vectors'
+    // maxima: 64 rows, k = 8: 11.7 and 63.5 us; 96 rows, k = 8: 12.7 and 15.6 us; 128 rows, k = 8, not taken: 13.0 and 12.4 us.)
+    if (BIAS || a.ngroups > 1 || (a.wide && 2 * a.nrows < 3 * N * (a.k + 1))) {
         // every 2 G-th row, so that a group's rows fall to as many maxima as there are
         top0 = top1 = -INFINITY;
         int e = sub;

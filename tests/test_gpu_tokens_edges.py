@@ -363,6 +363,36 @@ def test_route_gradient_of_tiny_and_large_scales(cuda_device, score, scale, E):
     close(got, want, grad_tolerance(xs, S, w, g, want, True, scale, "fp32"), "routeGrad at scale %g" % scale)
 
 
+@pytest.mark.parametrize("dtype", ["fp32", "bf16", "fp16"])
+@pytest.mark.parametrize("E,k", [(16, 1), (32, 4), (48, 6), (64, 8), (96, 8), (96, 12), (128, 16), (160, 20), (256, 32), (512, 32)])
+def test_route_of_few_vectors(cuda_device, dtype, E, k):
+    """Aligned columns with about as many 16-byte vectors as picks: right, and in the time of columns that are read one
+    element at a time or so.  When they all went the long way in 64 bits they took two to five times that."""
+    rng = np.random.default_rng(E + k)
+    check_route(1.5 * rng.standard_normal((200, E)), dtype, cuda_device, k)
+    x = (1.5 * torch.randn((65536, E + 8), device=cuda_device)).to(DT[dtype])
+    wide = matrix(x[:, :E].contiguous())
+    if dtype == "fp32":                                     # another base address, which is not that of a vector
+        flat = torch.empty(wide.t.numel() + 1, device=cuda_device)
+        narrow = matrix(flat[1:].view(wide.t.shape).copy_(wide.t))
+    else:
+        narrow = matrix(x[:, 1:E + 1])
+
+    def time(X):
+        times = []
+        for _ in range(12):
+            a, b = torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
+            a.record()
+            for _ in range(8):
+                tokens.route(X, k)
+            b.record()
+            torch.cuda.synchronize()
+            times.append(a.elapsed_time(b))
+        return min(times)
+
+    assert any(time(wide) < 2.0 * time(narrow) for _ in range(3))
+
+
 # ------------------------------------------------------------------------------------------ several at once
 
 def test_calls_of_different_sizes_from_two_host_threads(cuda_device):
