@@ -589,7 +589,9 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     if (a.renorm) {
 #pragma unroll
         for (int o = G / 2; o; o >>= 1) wsum += __shfl_xor_sync(0xffffffffu, wsum, o);
-        if (!(wsum > 1e-30f) && !none && !bad) again = true;            // sigmoids that leave the range of fp32
+        // Scores that leave the range of fp32, or come near enough to its end to lose bits that the sum of the picks, small
+        // itself, would bring back into the weights.
+        if ((!(wsum > 1e-30f) || (pick != 0 && w < 1e-31f && wsum < 1e-7f)) && !none && !bad) again = true;
     } else if (!softmax && pick != 0 && !bad && w < 1e-30f) {
         again = true;
     }

@@ -393,6 +393,24 @@ def test_route_of_few_vectors(cuda_device, dtype, E, k):
     assert any(time(wide) < 2.0 * time(narrow) for _ in range(3))
 
 
+@pytest.mark.parametrize("score", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("E,k", [(12, 3), (40, 6), (300, 16)])
+def test_route_weights_of_tiny_scores(cuda_device, score, E, k):
+    """Picks that are all tiny, forced by a bias (softmax) or for want of better ones (sigmoid), some of them next to the end
+    of fp32's range: their shares are still those of 64 bits."""
+    rng = np.random.default_rng(E)
+    x = np.full((64, E), -np.inf)
+    at = np.linspace(-100, -20, 64)
+    x[:, :k] = at[:, None] - 25.0 * rng.random((64, k))
+    bias = None
+    if score == "softmax":
+        x[:, k] = 0.0
+        bias = np.zeros(E)
+        bias[:k] = 4.0 + 0.125 * np.arange(k)
+    check_route(x, "fp32", cuda_device, k, score=score, bias=bias)
+    check_route(x, "fp32", cuda_device, k, score=score, bias=bias, scale=2.5)
+
+
 # ------------------------------------------------------------------------------------------ several at once
 
 def test_calls_of_different_sizes_from_two_host_threads(cuda_device):
