@@ -138,20 +138,16 @@ template <typename T> __device__ __noinline__ unsigned go_through(TopShared &sh,
     constexpr int N = Pack<T>::N, PER = kBatch / N;         // vectors per batch
     const int n = sh.set_aside;
     Entry from = bound == 0xffffffffu ? ~(Entry)0 : (Entry)(bound + 1) << 32;
-    int length = sh.length;                                 // nobody adds to the list before the barrier below
     for (int first = 0; first < n; first += PER) {
-        __syncthreads();                                    // every thread has read the same length, so all cut or none does
-        if (length > kList - kBatch) from = max(from, cut(sh, k));
+        // All threads cut or none does.  Some may read the length before others have added to it, but the last to add reads all
+        // of it; and nobody adds again before every thread has read it.
+        if (__syncthreads_or(sh.length > kList - kBatch)) from = max(from, cut(sh, k));
         const int last = min(n, first + PER);
         for (int i = first * N + (int)threadIdx.x; i < last * N; i += kTop) {
             const unsigned key = order_key(to_float(reinterpret_cast<const T *>(sh.aside)[i]));
             const int row = row0 + sh.aside_at[i / N] * N + (i & (N - 1));
             const Entry e = entry_of(key, (unsigned)row);
             if (e >= from && row >= 0 && row < rows) sh.list[atomicAdd(&sh.length, 1)] = e;
-        }
-        if (last < n) {
-            __syncthreads();                                // this batch is in the list
-            length = sh.length;
         }
     }
     __syncthreads();
