@@ -7,7 +7,9 @@
 //   d(w loss)/dx_v = w/t (P exp(x_v/t - L) - p_v)
 // The second form of the loss keeps the difference z - x, so it stays exact where the two agree; z is taken relative to the
 // entries' largest, x to the largest logit at an entry, so that neither loses anything where all are masked by a large number.
-// Masses and the loss are in fp64; exponentials over the rows, their sums and the gradient are in fp32.
+// Masses and the loss are in fp64; exponentials over the rows, their sums and the gradient are in fp32.  So is the gradient at a
+// column's first 128 entries, which a warp has in registers with their masses (fp64 there would make the chain that the other
+// warps wait for longer); further entries, and those of a row that comes twice, are gone through again in fp64.
 //
 // All three functions are bound by memory: one read of X, for the gradient one write of dX.
 #include <cuda_runtime.h>
@@ -599,7 +601,7 @@ cudaError_t launch_distill(const DistillArgs &a, int ncols, const void *X, void 
     const bool small = bytes <= kShortBytes;
     const long long part_bytes = MODE == GRAD ? kGradBytes : kBothBytes;
     long long parts = (bytes + part_bytes - 1) / part_bytes;
-    const long long fill = (296 + ncols - 1) / ncols, worth = (nvec + (small ? 63 : 255)) / (small ? 64 : 256);
+    const long long fill = (2 * kSMs + ncols - 1) / ncols, worth = (nvec + (small ? 63 : 255)) / (small ? 64 : 256);
     if (parts < fill) parts = fill < worth ? fill : worth;
     if (parts > most) parts = most;
     if (small) return launch_part<T, 64, MODE>(a, ncols, (int)parts, nvec, X, dX, st);
@@ -608,10 +610,10 @@ cudaError_t launch_distill(const DistillArgs &a, int ncols, const void *X, void 
 }
 
 // Without a gradient nothing has to stay on the chip, and a CTA is best kept on one column as long as there are
-// enough of them (131072 x 2048 bf16: 88 us in one part, 87 us in two, 95 us in three, 102 us in five).
+// enough of them, six per SM (131072 x 2048 bf16: 88 us in one part, 87 us in two, 95 us in three, 102 us in five).
 template <typename T> cudaError_t launch_loss(const DistillArgs &a, int ncols, const void *X, cudaStream_t st) {
     const long long bytes = (long long)a.nrows * (long long)sizeof(T);
-    const long long fill = 888 / ncols, worth = (bytes + 8191) / 8192;      // six per SM
+    const long long fill = 6 * kSMs / ncols, worth = (bytes + 8191) / 8192;
     long long parts = fill < worth ? fill : worth;
     if (parts < 1) parts = 1;
     if (parts > 8) parts = 8;

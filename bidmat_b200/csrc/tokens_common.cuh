@@ -57,6 +57,9 @@ __device__ __forceinline__ double warp_max(double v) {
 // Rows, columns and entries are counted in ints, with room for the steps of a loop.
 constexpr int kMostRows = 0x7fff0000, kMostEntries = 0x7fff0000;
 
+// How many CTAs fill the machine is counted in its SMs: this library is built for one part.
+constexpr int kSMs = 148;
+
 inline size_t dtype_size(int dtype) { return dtype == BIDMAT_B200_F32 ? 4 : 2; }
 inline bool dtype_ok(int dtype) { return dtype == BIDMAT_B200_F32 || dtype == BIDMAT_B200_BF16 || dtype == BIDMAT_B200_F16; }
 

@@ -323,7 +323,7 @@ __global__ void __launch_bounds__(kTop, LSE ? 3 : 4) top_kernel(TopArgs a, int g
 // CTA's longer way (100003 x 257 fp16: 28 us in one part, 43 us in three).
 template <typename T> cudaError_t launch_top(const TopArgs &a, const void *X, cudaStream_t st) {
     const long long bytes = (long long)a.nrows * (long long)sizeof(T);
-    const long long fill = 444 / a.ncols, worth = (bytes + 8191) / 8192;
+    const long long fill = 3 * kSMs / a.ncols, worth = (bytes + 8191) / 8192;
     long long parts = fill < worth ? fill : worth;
     if (parts < 1) parts = 1;
     if (parts > 8) parts = 8;
