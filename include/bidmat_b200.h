@@ -400,7 +400,8 @@ BIDMAT_B200_API int bidmat_b200_check_structure(int m, int ncols, int nnz, const
  *   key  = s + bias[row]; with bias == NULL the order of the scores themselves.  The bias takes part in
  *          the choice only, not in the weights;
  *   groups: ngroups equal groups of consecutive rows.  A group counts as the sum of its `grouptop` (1 or
- *          2) best s + bias; only the rows of the `topgroups` best groups compete (ties: lower group);
+ *          2) best s + bias; only the rows of the `topgroups` best groups compete (ties: lower group).  With
+ *          bias == NULL and grouptop == 1 that is again the order of the scores themselves;
  *   weight = s of the picked row, divided by the sum over the picked rows if renorm != 0, times scale.
  * Entries come in descending order of their keys, equal keys by ascending row; keys are compared as in
  * 64 bits.  A score or bias of -infinity (or a NaN bias) takes a row out; when fewer than k rows are
@@ -430,7 +431,8 @@ BIDMAT_B200_API int bidmat_b200_route_grad(int nrows, int ncols, int nnz, const 
 /* The k largest logits of every column of X(nrows x ncols) as a sparse matrix S(nrows x ncols) with k
  * entries per column (arrays as in bidmat_b200_route): the rows and the logits themselves, in descending
  * order, equal logits by ascending row; NaN counts as larger than any number, -0 as equal to 0.
- * lse (ncols values, may be NULL) receives log sum_v exp(X[v]/temperature) of every column.
+ * lse (ncols values, may be NULL) receives log sum_v exp(X[v]/temperature) of every column: -infinity for
+ * a column of -infinity, NaN for one with a NaN or +infinity.
  * 1 <= k <= BIDMAT_B200_TOP_MAX_K, k <= nrows; temperature is a finite normal number > 0; nrows and
  * ncols are at most 2^31 - 65536 here and in the functions below. */
 #define BIDMAT_B200_TOP_MAX_K 512
@@ -453,8 +455,10 @@ BIDMAT_B200_API int bidmat_b200_top_logits(int nrows, int ncols, const void *X, 
  * weights == NULL stands for ones.  Columns without an entry above -infinity have loss and gradient 0,
  * whatever Zlse says (bidmat_b200_top_logits leaves -infinity there for such a teacher); so have
  * columns of weight 0 in the two functions that take weights, which do not read them.  An entry
- * whose row is outside the matrix makes its column's results NaN; a row that comes twice counts with the
- * sum of its p.  A NaN or +infinity among a column's logits, or a column of -infinity, makes its results
+ * whose row is outside the matrix makes its column's results NaN, whatever its value; a row that comes
+ * twice counts with the sum of its p.  Xlse is rounded to fp32, and what that takes from it, 2^-24 |Xlse| at
+ * most, is the relative error of exp(X[v]/t - Xlse) in distill_grad (1e-6 for logits of 20, 0.6 per cent for
+ * a column masked by -1e5 as a whole); distill_with_grad has the sum itself and no such error.  A NaN or +infinity among a column's logits, or a column of -infinity, makes its results
  * NaN (in fp32, so also in fp16 outputs; finite gradients above 65504 become infinite there).
  * nnz is at most 2^31 - 65536.  dX may be X (with the same ld). */
 BIDMAT_B200_API int bidmat_b200_distill(int nrows, int ncols, int nnz, const void *X, long long ldx, int dtype,
