@@ -252,6 +252,30 @@ __device__ __forceinline__ bool near(float a, float b, float within) {
     return !(fabsf(a - b) > within + kNearPart * fmaxf(fabsf(a), fabsf(b)));
 }
 
+template <typename T> __device__ __forceinline__ bool same_numbers(const T *x, const float *bias, int r, int t) {
+    return to_float(x[r]) == to_float(x[t]) && bias[r] == bias[t];
+}
+
+// Whether behind the k picks is a row that may come before the last one: in the list of n, whose keys descend, the one with the
+// largest key that does not reach the bound, or one of those that equal `bound` (if not -infinity) and found no room in the list.
+// A lane looks at every G-th.
+template <typename T, int G>
+__device__ __noinline__ bool another_near(const Entry *sorted, int n, int k, const T *x, const float *bias, float within, float rejected,
+                                          float bound, const float *val, int nrows) {
+    const int sub = threadIdx.x & (G - 1);
+    const Entry last = sorted[k - 1];
+    for (int j = k + sub; j < n; j += G) {
+        const Entry q = sorted[j];
+        if (!near(key_of(last), key_of(q), within)) break;
+        if (!same_numbers(x, bias, row_of(last), row_of(q))) return true;
+    }
+    if (rejected > -INFINITY && near(key_of(last), rejected, within)) return true;
+    if (bound > -INFINITY && near(key_of(last), bound, within))
+        for (int e = sub; e < nrows; e += G)
+            if (val[e] == bound && !same_numbers(x, bias, row_of(last), e)) return true;
+    return false;
+}
+
 template <typename T, int G, bool BIAS>
 __global__ void __launch_bounds__(kRouteWarps * 32, 8)
 route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bias) {
@@ -265,7 +289,6 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     char *const base = reinterpret_cast<char *>(route_smem) + (size_t)warp * a.warp_bytes;
     float *val = reinterpret_cast<float *>(base) + which * a.stride;
     float *gval = val + ((a.nrows + 3) & ~3);
-    float *goff = gval + a.ngroups;                 // BIAS: what the roundings of a group's sum may come to
     Entry *list = reinterpret_cast<Entry *>(base + a.lists_at) + which * 2 * L, *sorted = list + L;
     const bool on = c < a.ncols;
     const T *x = X + (on ? c : 0) * a.ldx;
@@ -345,6 +368,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     if (a.ngroups > 1) {
         // a lane takes whole groups, four rows at once where that divides them; groups that would meet in one bank are begun at
         // another place in every lane
+        float *goff = gval + a.ngroups;             // BIAS: what the roundings of a group's sum may come to
         const int size = a.gsize, four = (size & 3) ? 0 : size / 4;
         auto first_of = [&](int g) { return (size & 31) ? 0 : g % four; };
         for (int g = sub; g < a.ngroups; g += G) {
@@ -384,7 +408,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
                 const float u = gval[h];
                 before += u > v || (u == v && h < g);
             }
-            const float off = BIAS ? goff[g] : kNearPart * fabsf(v);
+            const float off = BIAS ? goff[g] : 0.f;
             if (before < a.topgroups) worst = fminf(worst, v - off);
             else best = fmaxf(best, v > -INFINITY ? v + off : v), drop |= 1u << (n & 31);
         }
@@ -394,7 +418,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
             worst = fminf(worst, __shfl_xor_sync(0xffffffffu, worst, o));
             best = fmaxf(best, __shfl_xor_sync(0xffffffffu, best, o));
         }
-        groups_again = (BIAS || group_scores) && best > -INFINITY && !(worst - best > within);
+        groups_again = (BIAS || group_scores) && best > -INFINITY && (BIAS ? !(worst - best > within) : near(worst, best, within));
         n = 0;
         for (int g = sub; g < a.ngroups; g += G, n++) {
             if (!((drop >> (n & 31)) & 1u)) continue;
@@ -483,7 +507,7 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
     }
     int n = __shfl_sync(0xffffffffu, at, G - 1, G);
     at -= own;
-    bool left_out = false;                          // rows whose keys equal the bound in fp32 but are not all made of the same numbers
+    bool left_out = false;                          // rows whose keys equal the bound in fp32
     if (__any_sync(0xffffffffu, n > L)) {
         // more than the list holds: those above the bound, and of those that equal it the lowest rows
         const bool over = n > L;
@@ -498,19 +522,15 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         const int first = n1 - own1;
         n1 = __shfl_sync(0xffffffffu, n1, G - 1, G);
         if (over && n1 + a.k > L) again = true;     // one lane has too many of the largest
-        int taken = n1, first_tie = -1;
+        int taken = n1;
         for (int e = sub; e - sub < a.nrows; e += G) {
             const bool tie = over && !again && e < a.nrows && val[e] == bound;
             const unsigned vote = (__ballot_sync(0xffffffffu, tie) & mine) >> (which * G);
             const int to = taken + __popc(vote & before_me);
             if (tie && to < L) list[to] = entry_of(bound, e);
             taken += __popc(vote);
-            if (BIAS && vote) {
-                if (first_tie < 0) first_tie = e - sub + __ffs(vote) - 1;
-                if (tie && (to_float(x[e]) != to_float(x[first_tie]) || bias[e] != bias[first_tie])) left_out = true;
-            }
         }
-        left_out = left_out && taken > L;
+        left_out = taken > L;
         if (over) {
             mask = again ? 0 : above;
             at = first;
@@ -558,24 +578,20 @@ route_kernel(RouteArgs a, const T *__restrict__ X, const float *__restrict__ bia
         // numbers as the last pick there may be others.
 #pragma unroll
         for (int o = G / 2; o; o >>= 1) rejected = fmaxf(rejected, __shfl_xor_sync(0xffffffffu, rejected, o));
-        auto same_numbers = [&](Entry p, Entry q) {
-            const int r = row_of(p), t = row_of(q);
-            return to_float(x[r]) == to_float(x[t]) && bias[r] == bias[t];
-        };
-        if (pick != 0 && sub + 1 < min(a.k, n)) {
-            const Entry q = sorted[sub + 1];
-            if (near(key_of(pick), key_of(q), within) && !same_numbers(pick, q)) again = true;
-        }
-        if (n >= a.k) {
-            const Entry last = sorted[a.k - 1];
-            for (int j = a.k + sub; j < n; j += G) {
-                const Entry q = sorted[j];
-                if (!near(key_of(last), key_of(q), within)) break;
-                if (!same_numbers(last, q)) again = true;
+        bool further = left_out;
+        if (pick != 0) {
+            if (sub + 1 < n) {
+                const Entry q = sorted[sub + 1];
+                if (near(key_of(pick), key_of(q), within)) {
+                    if (!same_numbers(x, bias, row_of(pick), row_of(q))) again = true;
+                    else if (sub + 1 == a.k) further = true;
+                }
+            } else if (rejected > -INFINITY && near(key_of(pick), rejected, within)) {
+                again = true;
             }
-            if (rejected > -INFINITY && near(key_of(last), rejected, within)) again = true;
-            if (left_out && near(key_of(last), bound, within)) again = true;
         }
+        if (__any_sync(0xffffffffu, further) && n >= a.k)       // few columns
+            again |= another_near<T, G>(sorted, n, a.k, x, bias, within, rejected, left_out ? bound : -INFINITY, val, a.nrows);
     }
     const unsigned redo_groups = __ballot_sync(0xffffffffu, groups_again && !bad && on);
     const bool relative = softmax && !total;        // only the picks matter: relative to the largest of them
