@@ -236,7 +236,7 @@ __device__ __forceinline__ float key_of(Entry e) { return order_value((unsigned)
 
 // G lanes have a column, each every G-th of its rows.  The (k+1)-th largest of the lanes' maxima is a bound that k + 1
 // rows reach; few more do, so the rows that reach it are listed and each is ranked by counting the ones before it.
-// (256 x 4096 fp32 with bias and groups: 9.2 us, 36 us with sorted lists in the lanes' registers that are joined by exchanges;
+// (256 x 4096 fp32 with bias and groups: 9.8 us, 36 us with sorted lists in the lanes' registers that are joined by exchanges;
 // 160 x 65537 bf16 with groups: 36 and 47 us.)
 //
 // Where the order is that of scores plus bias, or of groups by their scores, it is found in fp32 first.  A sigmoid

@@ -14,8 +14,8 @@
 //   3. In the end the parts of a cluster are put together in its first CTA; what the k-th largest entry leaves (k, or a
 //      few more) goes to the place that its rank gives.
 // With many long columns the exponentials of the log-sum-exp and the steps between the rounds share the time with the
-// reading (131072 x 2048 bf16, k = 64: 159 us with the log-sum-exp, 112 us without, 82 us to read), with few columns the chain
-// of the steps counts (32768 x 1 fp32, k = 40: 9.2 us).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
+// reading (131072 x 2048 bf16, k = 64: 160 us with the log-sum-exp, 112 us without, 82 us to read), with few columns the chain
+// of the steps counts (32768 x 1 fp32, k = 40: 9.4 us).  Parts kept in shared memory and bounded each by itself took 517 us and 14 us: short-lived
 // CTAs spent most of their time on the bounds and on waiting for the cluster.
 #include <cuda_runtime.h>
 
